@@ -6,7 +6,7 @@ caller gets an exception.  Build with ``make -C gtg-vae_amd/csrc`` (or
 """
 import ctypes
 import os
-from ctypes import c_float, c_int, c_int64, c_size_t, c_void_p
+from ctypes import c_double, c_float, c_int, c_int64, c_size_t, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "csrc", "libgtgvae_hip.so")
@@ -19,6 +19,11 @@ class GtgError(RuntimeError):
 
 
 _P = c_void_p
+# argument groups of the entry points on rows of logits: (logits, dtype, rows, vocab, ld), then what each loss takes
+_LOGITS = [_P, c_int, c_int64, c_int, c_int64]
+_DISTILL = [_P, c_int64, _P, c_int, _P, c_int, _P, c_double, c_double]
+_POLICY = [_P, c_int64, _P, _P, _P, c_int64, _P] + [c_double] * 5
+_PAIRS = [_P, c_int, c_int64, c_int64, c_int, c_int64, c_int, _P, c_int64, _P]
 _SIGS = {
     "gtg_version": (c_int, []),
     "gtg_last_error": (ctypes.c_char_p, []),
@@ -73,6 +78,16 @@ _SIGS = {
     "gtg_embed_dropout_bwd": (c_int, [_P, _P, c_int64, c_int64, c_int, c_float, ctypes.c_uint64, ctypes.c_uint64, _P, _P,
                                       c_int, _P, c_size_t, _P]),
     "gtg_dropout": (c_int, [_P, c_int64, c_float, ctypes.c_uint64, ctypes.c_uint64, _P, _P]),
+    "gtg_top_logits": (c_int, _LOGITS + [c_int, c_double] + [_P] * 4),
+    "gtg_token_logprob_fwd": (c_int, _LOGITS + [_P, c_int64, c_double] + [_P] * 4),
+    "gtg_token_logprob_bwd": (c_int, _LOGITS + [_P, c_int64, c_double] + [_P] * 4 + [c_int64, _P]),
+    "gtg_distill_loss_fwd": (c_int, _LOGITS + _DISTILL + [c_int] + [_P] * 4 + [c_int64, _P]),
+    "gtg_distill_loss_bwd": (c_int, _LOGITS + _DISTILL + [_P] * 3 + [c_int, _P, c_int64, _P]),
+    "gtg_policy_loss_fwd": (c_int, _LOGITS + _POLICY + [c_int] + [_P] * 6 + [c_int64, _P]),
+    "gtg_policy_loss_bwd": (c_int, _LOGITS + _POLICY + [_P] * 3 + [c_int, _P, c_int64, _P]),
+    "gtg_preference_workspace_bytes": (c_size_t, [c_int64, c_int64]),
+    "gtg_preference_fwd": (c_int, _PAIRS + [_P, c_double, c_double, c_int] + [_P] * 6 + [c_size_t, _P]),
+    "gtg_preference_bwd": (c_int, _PAIRS + [_P] * 5 + [c_int64, _P]),
     "gtg_adam_step": (c_int, [_P] * 4 + [c_int64, _P, c_float, c_float, c_float, c_float, c_float, _P]),
     "gtg_adam_update": (c_int, [_P] * 4 + [c_int64, _P, c_float, c_float, c_float, c_float, _P]),
     "gtg_gemm_f32": (c_int, [_P, _P, _P] + [c_int] * 8 + [_P, c_int, _P, c_int, _P, c_size_t, c_int, _P]),

@@ -11,6 +11,7 @@
 #include <string.h>
 
 #include <atomic>
+#include <cmath>
 #include <map>
 #include <mutex>
 #include <string>
@@ -1427,6 +1428,211 @@ int gtg_proj_ce_bwd(const float* W, const float* gloss, const int32_t* rowmap, c
         GTG_TRY(ce_rows(2, dHc, gloss, rowmap, rows, k, dH, s));
     }
     return GTG_OK;
+}
+
+// ---- losses and read-outs on rows of vocabulary logits --------------------------
+static size_t dtype_size(int dtype) { return dtype == GTG_DTYPE_F32 ? 4 : (dtype == GTG_DTYPE_F16 || dtype == GTG_DTYPE_BF16) ? 2 : 0; }
+static bool aligned_to(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+
+#define GTG_REQUIRE_LOGITS(logits, dtype, rows, vocab, ld)                                                              \
+    do {                                                                                                                \
+        GTG_REQUIRE(dtype_size(dtype) != 0, "dtype must be GTG_DTYPE_F32, _F16 or _BF16");                              \
+        GTG_REQUIRE((rows) >= 0 && (rows) <= 0x7fffffff && (vocab) >= 1, "bad size");                                   \
+        GTG_REQUIRE((ld) >= (vocab), "the row stride must be at least vocab");                                          \
+        GTG_REQUIRE((rows) == 0 || ((logits) && aligned_to(logits, dtype_size(dtype))), "logits: null or misaligned"); \
+    } while (0)
+#define GTG_REQUIRE_GRADIENT(logits, dtype, rows, vocab, dlogits, ldg)                                                    \
+    do {                                                                                                                  \
+        GTG_REQUIRE((ldg) >= (vocab), "the gradient's row stride must be at least vocab");                                \
+        GTG_REQUIRE((rows) == 0 || ((dlogits) && aligned_to(dlogits, dtype_size(dtype))), "dlogits: null or misaligned"); \
+        GTG_REQUIRE((rows) == 0 || (dlogits) != (logits), "dlogits must not overlap the logits");                         \
+    } while (0)
+
+int gtg_top_logits(const void* logits, int dtype, int64_t rows, int vocab, int64_t ld, int k, double temperature,
+                   void* values, int32_t* indices, float* tail, void* stream)
+{
+    GTG_REQUIRE_LOGITS(logits, dtype, rows, vocab, ld);
+    GTG_REQUIRE(k >= 1 && k <= 256 && k <= vocab, "k must be in [1, min(vocab, 256)]");
+    GTG_REQUIRE(temperature > 0 && std::isfinite(temperature), "temperature must be positive");
+    if (rows == 0) return GTG_OK;
+    GTG_REQUIRE(values && indices && tail, "null pointer");
+    GTG_REQUIRE(aligned_to(values, dtype_size(dtype)), "values: misaligned");
+    return top_logits(logits, dtype, rows, vocab, ld, k, temperature, values, indices, tail, (hipStream_t)stream);
+}
+
+int gtg_token_logprob_fwd(const void* logits, int dtype, int64_t rows, int vocab, int64_t ld, const int64_t* targets,
+                          int64_t padidx, double temperature, float* logp, float* entropy, float* stats, void* stream)
+{
+    GTG_REQUIRE_LOGITS(logits, dtype, rows, vocab, ld);
+    GTG_REQUIRE(temperature > 0 && std::isfinite(temperature), "temperature must be positive");
+    if (rows == 0) return GTG_OK;
+    GTG_REQUIRE(targets && logp && entropy, "null pointer");
+    GTG_REQUIRE(stats == nullptr || aligned_to(stats, 16), "stats: misaligned");
+    const TokenRows t{logits, dtype, rows, vocab, ld, targets, padidx, nullptr};
+    return token_logprob_fwd(t, temperature, logp, entropy, stats, nullptr, (hipStream_t)stream);
+}
+
+int gtg_token_logprob_bwd(const void* logits, int dtype, int64_t rows, int vocab, int64_t ld, const int64_t* targets,
+                          int64_t padidx, double temperature, const float* stats, const float* g_logp,
+                          const float* g_entropy, void* dlogits, int64_t ldg, void* stream)
+{
+    GTG_REQUIRE_LOGITS(logits, dtype, rows, vocab, ld);
+    GTG_REQUIRE_GRADIENT(logits, dtype, rows, vocab, dlogits, ldg);
+    GTG_REQUIRE(temperature > 0 && std::isfinite(temperature), "temperature must be positive");
+    if (rows == 0) return GTG_OK;
+    GTG_REQUIRE(targets && stats && aligned_to(stats, 16), "null or misaligned pointer");
+    const TokenRows t{logits, dtype, rows, vocab, ld, targets, padidx, nullptr};
+    return token_logprob_bwd(t, temperature, stats, g_logp, g_entropy, nullptr, nullptr, 0, 1, dlogits, ldg, (hipStream_t)stream);
+}
+
+static const char* distill_fault(int vocab, const void* values, int value_dtype, const int32_t* indices, int k, double temperature,
+                                 double ce_weight, int64_t rows)
+{
+    if (dtype_size(value_dtype) == 0) return "value_dtype must be GTG_DTYPE_F32, _F16 or _BF16";
+    if (k < 1 || k > 256) return "k must be in [1, 256]";
+    if (vocab > distill_max_vocab()) return "vocab must be at most 400 000";
+    if (!(temperature > 0) || !std::isfinite(temperature)) return "temperature must be positive";
+    if (!(ce_weight >= 0 && ce_weight <= 1)) return "ce_weight must be in [0, 1]";
+    if (rows > 0 && (!values || !indices || !aligned_to(values, dtype_size(value_dtype)))) return "null or misaligned pointer";
+    return nullptr;
+}
+
+int gtg_distill_loss_fwd(const void* logits, int dtype, int64_t rows, int vocab, int64_t ld, const int64_t* targets,
+                         int64_t padidx, const void* values, int value_dtype, const int32_t* indices, int k,
+                         const float* tail, double temperature, double ce_weight, int reduction, double* norm,
+                         float* row_loss, float* loss, void* dlogits, int64_t ldg, void* stream)
+{
+    GTG_REQUIRE_LOGITS(logits, dtype, rows, vocab, ld);
+    if (dlogits) GTG_REQUIRE_GRADIENT(logits, dtype, rows, vocab, dlogits, ldg);
+    if (const char* fault = distill_fault(vocab, values, value_dtype, indices, k, temperature, ce_weight, rows))
+        return set_error(GTG_ERR_INVALID, "%s: %s", __func__, fault);
+    GTG_REQUIRE(reduction >= GTG_REDUCE_NONE && reduction <= GTG_REDUCE_MEAN, "reduction must be GTG_REDUCE_NONE, _SUM or _MEAN");
+    GTG_REQUIRE(rows == 0 || (targets && row_loss), "null pointer");
+    GTG_REQUIRE(reduction == GTG_REDUCE_NONE || loss, "null pointer");
+    GTG_REQUIRE(reduction != GTG_REDUCE_MEAN || norm, "null pointer");
+    hipStream_t s = (hipStream_t)stream;
+    const TokenRows t{logits, dtype, rows, vocab, ld, targets, padidx, nullptr};
+    if (reduction != GTG_REDUCE_MEAN) norm = nullptr;
+    if (norm) GTG_TRY(count_rows(t, norm, s));
+    if (rows > 0) {
+        const DistillRows d{values, value_dtype, indices, k, tail, temperature, ce_weight};
+        GTG_TRY(distill_rows(t, d, nullptr, nullptr, norm, false, row_loss, dlogits, ldg, s));
+    }
+    return reduction == GTG_REDUCE_NONE ? GTG_OK : total_loss(row_loss, rows, norm, loss, s);
+}
+
+int gtg_distill_loss_bwd(const void* logits, int dtype, int64_t rows, int vocab, int64_t ld, const int64_t* targets,
+                         int64_t padidx, const void* values, int value_dtype, const int32_t* indices, int k,
+                         const float* tail, double temperature, double ce_weight, const double* norm, const float* gloss,
+                         const float* gscale, int unless_unit, void* dlogits, int64_t ldg, void* stream)
+{
+    GTG_REQUIRE_LOGITS(logits, dtype, rows, vocab, ld);
+    GTG_REQUIRE_GRADIENT(logits, dtype, rows, vocab, dlogits, ldg);
+    if (const char* fault = distill_fault(vocab, values, value_dtype, indices, k, temperature, ce_weight, rows))
+        return set_error(GTG_ERR_INVALID, "%s: %s", __func__, fault);
+    GTG_REQUIRE(!unless_unit || gscale, "unless_unit needs gscale");
+    if (rows == 0) return GTG_OK;
+    GTG_REQUIRE(targets != nullptr, "null pointer");
+    const TokenRows t{logits, dtype, rows, vocab, ld, targets, padidx, nullptr};
+    const DistillRows d{values, value_dtype, indices, k, tail, temperature, ce_weight};
+    return distill_rows(t, d, gloss, gscale, norm, unless_unit != 0, nullptr, dlogits, ldg, (hipStream_t)stream);
+}
+
+static const char* policy_fault(const PolicyRows& p, const int64_t* targets, int64_t rows)
+{
+    if (!(p.temperature > 0) || !std::isfinite(p.temperature)) return "temperature must be positive";
+    if (!(p.clip_low >= 0) || !(p.clip_high >= 0)) return "clip_low and clip_high must not be negative";
+    if (!std::isfinite(p.kl_coef) || !std::isfinite(p.entropy_coef)) return "kl_coef and entropy_coef must be finite";
+    if (rows > 0 && p.adv_rows < 1) return "adv_rows must be positive";
+    if (rows > 0 && (!targets || !p.old_logp || !p.advantages)) return "null pointer";
+    if (p.kl_coef != 0.0 && rows > 0 && !p.ref_logp) return "kl_coef needs ref_logp";
+    return nullptr;
+}
+
+int gtg_policy_loss_fwd(const void* logits, int dtype, int64_t rows, int vocab, int64_t ld, const int64_t* targets,
+                        int64_t padidx, const uint8_t* mask, const float* old_logp, const float* advantages,
+                        int64_t adv_rows, const float* ref_logp, double clip_low, double clip_high, double kl_coef,
+                        double entropy_coef, double temperature, int reduction, double* norm, float* row_loss,
+                        float* loss, float* logp, float* entropy, void* dlogits, int64_t ldg, void* stream)
+{
+    GTG_REQUIRE_LOGITS(logits, dtype, rows, vocab, ld);
+    if (dlogits) GTG_REQUIRE_GRADIENT(logits, dtype, rows, vocab, dlogits, ldg);
+    const PolicyRows p{old_logp, advantages, adv_rows, ref_logp, clip_low, clip_high, kl_coef, entropy_coef, temperature};
+    if (const char* fault = policy_fault(p, targets, rows)) return set_error(GTG_ERR_INVALID, "%s: %s", __func__, fault);
+    GTG_REQUIRE(reduction >= GTG_REDUCE_NONE && reduction <= GTG_REDUCE_MEAN, "reduction must be GTG_REDUCE_NONE, _SUM or _MEAN");
+    GTG_REQUIRE(rows == 0 || row_loss, "null pointer");
+    GTG_REQUIRE(reduction == GTG_REDUCE_NONE || loss, "null pointer");
+    GTG_REQUIRE(reduction != GTG_REDUCE_MEAN || norm, "null pointer");
+    hipStream_t s = (hipStream_t)stream;
+    const TokenRows t{logits, dtype, rows, vocab, ld, targets, padidx, mask};
+    if (reduction != GTG_REDUCE_MEAN) norm = nullptr;
+    if (norm) GTG_TRY(count_rows(t, norm, s));
+    if (rows > 0) GTG_TRY(policy_rows(t, p, nullptr, nullptr, norm, false, row_loss, logp, entropy, dlogits, ldg, s));
+    return reduction == GTG_REDUCE_NONE ? GTG_OK : total_loss(row_loss, rows, norm, loss, s);
+}
+
+int gtg_policy_loss_bwd(const void* logits, int dtype, int64_t rows, int vocab, int64_t ld, const int64_t* targets,
+                        int64_t padidx, const uint8_t* mask, const float* old_logp, const float* advantages,
+                        int64_t adv_rows, const float* ref_logp, double clip_low, double clip_high, double kl_coef,
+                        double entropy_coef, double temperature, const double* norm, const float* gloss,
+                        const float* gscale, int unless_unit, void* dlogits, int64_t ldg, void* stream)
+{
+    GTG_REQUIRE_LOGITS(logits, dtype, rows, vocab, ld);
+    GTG_REQUIRE_GRADIENT(logits, dtype, rows, vocab, dlogits, ldg);
+    const PolicyRows p{old_logp, advantages, adv_rows, ref_logp, clip_low, clip_high, kl_coef, entropy_coef, temperature};
+    if (const char* fault = policy_fault(p, targets, rows)) return set_error(GTG_ERR_INVALID, "%s: %s", __func__, fault);
+    GTG_REQUIRE(!unless_unit || gscale, "unless_unit needs gscale");
+    if (rows == 0) return GTG_OK;
+    const TokenRows t{logits, dtype, rows, vocab, ld, targets, padidx, mask};
+    return policy_rows(t, p, gloss, gscale, norm, unless_unit != 0, nullptr, nullptr, nullptr, dlogits, ldg, (hipStream_t)stream);
+}
+
+size_t gtg_preference_workspace_bytes(int64_t T, int64_t pairs)
+{
+    return T < 0 || pairs < 0 ? 0 : (size_t)(T + 1) * (size_t)(2 * pairs) * sizeof(double);
+}
+
+#define GTG_REQUIRE_PAIRS(T, pairs)                                                                                   \
+    GTG_REQUIRE((T) >= 0 && (pairs) >= 0 && (T) <= 0x7fffffff && (pairs) <= 0x3fffffff &&                             \
+                    ((T) == 0 || (pairs) <= 0x7fffffff / 2 / (T)), "bad size")
+
+int gtg_preference_fwd(const void* logits, int dtype, int64_t T, int64_t pairs, int vocab, int64_t ld, int batch_first,
+                       const int64_t* targets, int64_t padidx, const uint8_t* mask, const float* ref_logp, double beta,
+                       double label_smoothing, int reduction, float* stats, float* coef, float* seq_logp, float* pair_loss,
+                       float* loss, void* ws, size_t ws_bytes, void* stream)
+{
+    GTG_REQUIRE_PAIRS(T, pairs);
+    const int64_t rows = T * 2 * pairs;
+    GTG_REQUIRE_LOGITS(logits, dtype, rows, vocab, ld);
+    GTG_REQUIRE(std::isfinite(beta), "beta must be finite");
+    GTG_REQUIRE(label_smoothing >= 0 && label_smoothing < 1, "label_smoothing must be in [0, 1)");
+    GTG_REQUIRE(reduction >= GTG_REDUCE_NONE && reduction <= GTG_REDUCE_MEAN, "reduction must be GTG_REDUCE_NONE, _SUM or _MEAN");
+    GTG_REQUIRE(reduction == GTG_REDUCE_NONE || loss, "null pointer");
+    hipStream_t s = (hipStream_t)stream;
+    if (pairs == 0) return reduction == GTG_REDUCE_NONE ? GTG_OK : total_loss(nullptr, 0, nullptr, loss, s);
+    GTG_REQUIRE(ref_logp && coef && seq_logp && pair_loss && (rows == 0 || (targets && stats)), "null pointer");
+    GTG_REQUIRE(aligned_to(stats, 16), "stats: misaligned");
+    GTG_REQUIRE(ws && aligned_to(ws, 8) && ws_bytes >= gtg_preference_workspace_bytes(T, pairs), "workspace too small");
+    double* logp = reinterpret_cast<double*>(ws);
+    const TokenRows t{logits, dtype, rows, vocab, ld, targets, padidx, mask};
+    if (rows > 0) GTG_TRY(token_logprob_fwd(t, 1.0, nullptr, nullptr, stats, logp, s));
+    return prefer_pairs(logp, logp + rows, T, pairs, batch_first != 0, ref_logp, beta, label_smoothing, reduction == GTG_REDUCE_MEAN,
+                        seq_logp, coef, pair_loss, reduction == GTG_REDUCE_NONE ? nullptr : loss, s);
+}
+
+int gtg_preference_bwd(const void* logits, int dtype, int64_t T, int64_t pairs, int vocab, int64_t ld, int batch_first,
+                       const int64_t* targets, int64_t padidx, const uint8_t* mask, const float* stats, const float* coef,
+                       const float* gscale, const float* gloss, void* dlogits, int64_t ldg, void* stream)
+{
+    GTG_REQUIRE_PAIRS(T, pairs);
+    const int64_t rows = T * 2 * pairs;
+    GTG_REQUIRE_LOGITS(logits, dtype, rows, vocab, ld);
+    GTG_REQUIRE_GRADIENT(logits, dtype, rows, vocab, dlogits, ldg);
+    if (rows == 0) return GTG_OK;
+    GTG_REQUIRE(targets && stats && coef && aligned_to(stats, 16), "null or misaligned pointer");
+    const TokenRows t{logits, dtype, rows, vocab, ld, targets, padidx, mask};
+    return token_logprob_bwd(t, 1.0, stats, coef, nullptr, gscale, gloss, batch_first ? -T : 2 * pairs, pairs, dlogits, ldg,
+                             (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -343,6 +343,56 @@ size_t ce_bias_grad_workspace(int V);
 int ce_bias_grad(const float* P, int64_t ldp, int V, const float* g, const int32_t* rowmap, int64_t R, float* partial,
                  float* db, hipStream_t s);
 
+// ---- losses and read-outs on rows of logits (token_ops.hip) -------------------
+// Row r of the logits at logits + r ld (ld in elements); a row counts where targets[r] != padidx and mask[r] != 0.
+struct TokenRows {
+    const void* logits;
+    int dtype;  // GTG_DTYPE_*
+    int64_t rows;
+    int vocab;
+    int64_t ld;
+    const int64_t* targets;
+    int64_t padidx;
+    const uint8_t* mask;  // nullable
+};
+struct PolicyRows {
+    const float* old_logp;
+    const float* advantages;
+    int64_t adv_rows;  // advantages[r mod adv_rows]
+    const float* ref_logp;  // nullable
+    double clip_low, clip_high, kl_coef, entropy_coef, temperature;
+};
+struct DistillRows {
+    const void* values;
+    int value_dtype;
+    const int32_t* indices;
+    int k;
+    const float* tail;  // nullable
+    double temperature, ce_weight;
+};
+int top_logits(const void* logits, int dtype, int64_t R, int V, int64_t ld, int k, double temperature, void* values,
+               int32_t* indices, float* tail, hipStream_t s);
+// stats (rows, 4) and logp64 (rows) nullable
+int token_logprob_fwd(const TokenRows& t, double temperature, float* logp, float* entropy, float* stats, double* logp64,
+                      hipStream_t s);
+// the coefficient of row r's log-probability: g_logp[b] (* *gscale) (* gloss[b mod pairs]), b = r (group 0),
+// r mod group (group > 0) or r / -group (group < 0)
+int token_logprob_bwd(const TokenRows& t, double temperature, const float* stats, const float* g_logp, const float* g_entropy,
+                      const float* gscale, const float* gloss, int64_t group, int64_t pairs, void* dx, int64_t ldg,
+                      hipStream_t s);
+int count_rows(const TokenRows& t, double* norm, hipStream_t s);  // *norm = 1 / (rows that count), 0 if none
+int total_loss(const float* row_loss, int64_t R, const double* norm, float* loss, hipStream_t s);
+// row r's gradient is weighted with gloss[r] * *gscale * *norm (each 1 where NULL); skip_unit: the launch does nothing
+// where *gscale is 1
+int policy_rows(const TokenRows& t, const PolicyRows& p, const float* gloss, const float* gscale, const double* norm,
+                bool skip_unit, float* row_loss, float* logp, float* entropy, void* dx, int64_t ldg, hipStream_t s);
+int distill_max_vocab();
+int distill_rows(const TokenRows& t, const DistillRows& d, const float* gloss, const float* gscale, const double* norm,
+                 bool skip_unit, float* row_loss, void* dx, int64_t ldg, hipStream_t s);
+int prefer_pairs(const double* logp, double* seq, int64_t T, int64_t pairs, bool batch_first, const float* ref, double beta,
+                 double label_smoothing, bool mean, float* seq_logp, float* coef, float* pair_loss, float* loss,
+                 hipStream_t s);
+
 // ---- one-layer LSTM over a padded sequence (lstm.hip) ------------------------
 // x (T, B, I), w_ih (4H, I), w_hh (4H, H), biases (4H), h0 / c0 (B, H) nullable; hs / cs (T, B, H) and gates
 // (T, B, 4H) (the gate activations) are outputs and the backward's saved state.  I % 4 == 0, H % 64 == 0.

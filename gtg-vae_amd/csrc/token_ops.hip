@@ -1,0 +1,936 @@
+// Losses and read-outs on rows of vocabulary logits (fp32, fp16 or bf16), gfx950 only: the k largest logits of a row,
+// the log-probability of a row's token, and the distillation, policy and preference losses with their gradients.
+//
+// Every operator is a reduction over a row of V logits (a soft-max's maximum and sum and little else) followed, for a
+// gradient, by a map over the same row.  Each does a handful of operations per logit, so what bounds them is the row's
+// way through memory: V elements in, V elements out.  One block takes one row; sums are held in 32 bits, what is one
+// number per row (logarithms, ratios, losses) in 64.
+//
+// A row whose target is the pad symbol, or whose mask byte is zero, is not read: its outputs are zero.
+#include "gtg_internal.h"
+
+namespace gtg {
+namespace {
+
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2v __attribute__((ext_vector_type(2)));
+
+constexpr double LOG2E = 1.4426950408889634;
+__device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
+
+// 16 bytes of logits, element by element as fp32.
+struct F32 {
+    typedef float Store;
+    static constexpr int VEC = 4;
+    __device__ static float get(const u32x4& v, int q) { return __uint_as_float(v[q]); }
+    __device__ static void clear(u32x4& v, int q) { v[q] = 0xff800000u; }
+    __device__ static float load(const Store* p) { return *p; }
+    __device__ static Store cvt(float f) { return f; }
+    __device__ static u32x4 pack(const float* f)
+    {
+        u32x4 v;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] = __float_as_uint(f[q]);
+        return v;
+    }
+};
+struct BF16 {
+    typedef __bf16 Store;
+    static constexpr int VEC = 8;
+    __device__ static float get(const u32x4& v, int q)
+    {
+        return __uint_as_float((q & 1) ? (v[q >> 1] & 0xffff0000u) : (v[q >> 1] << 16));
+    }
+    __device__ static void clear(u32x4& v, int q)
+    {
+        v[q >> 1] = (q & 1) ? ((v[q >> 1] & 0xffffu) | 0xff800000u) : ((v[q >> 1] & 0xffff0000u) | 0xff80u);
+    }
+    __device__ static float load(const Store* p) { return (float)*p; }
+    __device__ static Store cvt(float f) { return (__bf16)f; }
+    __device__ static u32x4 pack(const float* f)
+    {
+        u32x4 v;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const f32x2 two = {f[2 * q], f[2 * q + 1]};
+            v[q] = __builtin_bit_cast(unsigned, __builtin_convertvector(two, bf16x2));
+        }
+        return v;
+    }
+};
+struct F16 {
+    typedef _Float16 Store;
+    static constexpr int VEC = 8;
+    __device__ static float get(const u32x4& v, int q)
+    {
+        return (float)__builtin_bit_cast(_Float16, (unsigned short)((q & 1) ? (v[q >> 1] >> 16) : (v[q >> 1] & 0xffffu)));
+    }
+    __device__ static void clear(u32x4& v, int q)
+    {
+        v[q >> 1] = (q & 1) ? ((v[q >> 1] & 0xffffu) | 0xfc000000u) : ((v[q >> 1] & 0xffff0000u) | 0xfc00u);
+    }
+    __device__ static float load(const Store* p) { return (float)*p; }
+    __device__ static Store cvt(float f) { return (_Float16)f; }
+    __device__ static u32x4 pack(const float* f)
+    {
+        u32x4 v;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const f32x2 two = {f[2 * q], f[2 * q + 1]};
+            v[q] = __builtin_bit_cast(unsigned, __builtin_convertvector(two, f16x2v));
+        }
+        return v;
+    }
+};
+
+// ---- a row and how a block of NT threads walks over it --------------------------------------------------------
+// The row is cut where 16-byte alignment begins and ends: up to VEC - 1 elements in front and behind, taken one each by
+// the first 2 VEC threads (`xe`, `je`), and the body of whole vectors between them, vector i by thread i mod NT.  No
+// access leaves the row, whatever its alignment and length.
+template <typename E, int NT>
+struct Row {
+    typedef typename E::Store S;
+    static constexpr int VEC = E::VEC;
+    const S* p;
+    int V, head, nb, je;  // elements in front, vectors in the body, this thread's single element or -1
+    float xe;             // its value, -inf if there is none
+
+    __device__ Row(const S* row, int vocab) : p(row), V(vocab)
+    {
+        const int off = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(S));
+        head = off ? VEC - off : 0;
+        if (head > V) head = V;
+        nb = (V - head) / VEC;
+        const int tail0 = head + nb * VEC, t = threadIdx.x;
+        je = t < head ? t : (t >= VEC && tail0 + t - VEC < V && t < 2 * VEC ? tail0 + t - VEC : -1);
+        xe = neg_inf();
+    }
+    __device__ void load_single() { if (je >= 0) xe = E::load(p + je); }
+    __device__ const u32x4* body() const { return reinterpret_cast<const u32x4*>(p + head); }
+    // f(index of the vector's first element, vector)
+    template <typename F>
+    __device__ __forceinline__ void each(F f) const
+    {
+        const u32x4* b = body();
+        for (int i = threadIdx.x; i < nb; i += NT) f(head + i * VEC, b[i]);
+    }
+};
+
+// A gradient row: vectors where its alignment is the logits' own, single elements otherwise.
+template <typename E>
+struct OutRow {
+    typename E::Store* p;
+    bool aligned;
+    __device__ OutRow(void* base, int64_t ld, int64_t r, const typename E::Store* in)
+        : p(reinterpret_cast<typename E::Store*>(base) + r * ld),
+          aligned(((reinterpret_cast<uintptr_t>(p) ^ reinterpret_cast<uintptr_t>(in)) & 15) == 0)
+    {
+    }
+    __device__ __forceinline__ void vec(int j, const float* f) const
+    {
+        if (aligned) {
+            *reinterpret_cast<u32x4*>(p + j) = E::pack(f);
+        } else {
+#pragma unroll
+            for (int q = 0; q < E::VEC; ++q) p[j + q] = E::cvt(f[q]);
+        }
+    }
+    __device__ __forceinline__ void one(int j, float f) const { p[j] = E::cvt(f); }
+};
+
+template <typename E, int NT>
+__device__ void fill_row(const Row<E, NT>& row, const OutRow<E>& out, float value)
+{
+    float f[E::VEC];
+#pragma unroll
+    for (int q = 0; q < E::VEC; ++q) f[q] = value;
+    for (int i = threadIdx.x; i < row.nb; i += NT) out.vec(row.head + i * E::VEC, f);
+    if (row.je >= 0) out.one(row.je, value);
+}
+
+// ---- reductions over a block ------------------------------------------------------------------------------------
+__device__ __forceinline__ float wave_max(float v)
+{
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+    return v;
+}
+__device__ __forceinline__ float wave_sum(float v)
+{
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+__device__ __forceinline__ double wave_sum(double v)
+{
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+
+template <int NT>
+__device__ __forceinline__ float block_max(float v, float* sh)
+{
+    v = wave_max(v);
+    if (NT == 64) return v;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = sh[0];
+#pragma unroll
+    for (int w = 1; w < NT / 64; ++w) v = fmaxf(v, sh[w]);
+    return v;
+}
+template <int NT>
+__device__ __forceinline__ float block_sum(float v, float* sh)
+{
+    v = wave_sum(v);
+    if (NT == 64) return v;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = sh[0];
+#pragma unroll
+    for (int w = 1; w < NT / 64; ++w) v += sh[w];
+    return v;
+}
+template <int NT>
+__device__ __forceinline__ int block_count(int v, int* sh)
+{
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o);
+    if (NT == 64) return v;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = sh[0];
+#pragma unroll
+    for (int w = 1; w < NT / 64; ++w) v += sh[w];
+    return v;
+}
+
+__device__ __forceinline__ float finite_or_zero(float m) { return m == neg_inf() ? 0.f : m; }
+// x - m, from below at the lowest finite number: its product with exp(-inf) = 0 is then 0 and not NaN
+__device__ __forceinline__ float clamped(float d) { return fmaxf(d, -3.402823466e38f); }
+
+// ---- which rows count -------------------------------------------------------------------------------------------
+struct Rows {
+    const void* x;       // logits, row r at x + r ld
+    int64_t ld;
+    int vocab;
+    const int64_t* targets;
+    int64_t pad;
+    const uint8_t* mask;  // nullable
+    __device__ __forceinline__ bool kept(int64_t r) const { return targets[r] != pad && (mask == nullptr || mask[r] != 0); }
+};
+
+// What a row's gradient is multiplied with: gloss[r], *gscale and *norm, each 1 where absent.
+struct Weight {
+    const float* gloss;
+    const float* gscale;
+    const double* norm;
+    __device__ __forceinline__ double of(int64_t r) const
+    {
+        return (gloss ? (double)gloss[r] : 1.0) * (gscale ? (double)*gscale : 1.0) * (norm ? *norm : 1.0);
+    }
+};
+
+// 1 / (rows that count), 0 if none does.
+__global__ __launch_bounds__(1024) void count_kernel(Rows rows, int64_t R, double* __restrict__ norm)
+{
+    __shared__ int sh[16];
+    int n = 0;
+    for (int64_t r = threadIdx.x; r < R; r += 1024) n += rows.kept(r) ? 1 : 0;
+    n = block_count<1024>(n, sh);
+    if (threadIdx.x == 0) *norm = n > 0 ? 1.0 / (double)n : 0.0;
+}
+
+// loss = (*norm or 1) * sum of row_loss, in 64 bits and a fixed order
+__global__ __launch_bounds__(1024) void total_kernel(const float* __restrict__ row_loss, int64_t R,
+                                                     const double* __restrict__ norm, float* __restrict__ loss)
+{
+    __shared__ double sh[16];
+    double s = 0.0;
+    for (int64_t r = threadIdx.x; r < R; r += 1024) s += (double)row_loss[r];
+    s = wave_sum(s);
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        s = 0.0;
+        for (int w = 0; w < 16; ++w) s += sh[w];
+        *loss = R > 0 ? (float)(s * (norm ? *norm : 1.0)) : 0.f;
+    }
+}
+
+// ---- maximum, sum of exponentials and their first moment ---------------------------------------------------------
+// m = max x, s = sum exp(c (x - m)) with c in powers of two, t = sum exp(c (x - m)) (x - m): all of the row, in every thread.
+template <typename E, int NT>
+__device__ __forceinline__ void row_stats(const Row<E, NT>& row, float c, float& m, float& s, float& t, float* sh)
+{
+    float mx = row.xe;
+    row.each([&](int, const u32x4& v) {
+#pragma unroll
+        for (int q = 0; q < E::VEC; ++q) mx = fmaxf(mx, E::get(v, q));
+    });
+    m = finite_or_zero(block_max<NT>(mx, sh));
+    const float me = m;
+    float ss = 0.f, tt = 0.f;
+    auto add = [&](float x) {
+        const float d = x - me, e = exp2f(d * c);
+        ss += e;
+        tt += e * clamped(d);
+    };
+    add(row.xe);
+    row.each([&](int, const u32x4& v) {
+#pragma unroll
+        for (int q = 0; q < E::VEC; ++q) add(E::get(v, q));
+    });
+    s = block_sum<NT>(ss, sh);
+    t = block_sum<NT>(tt, sh);
+}
+
+// ---- log-probability and entropy ---------------------------------------------------------------------------------
+// logp = x_y / tau - lse, entropy = log s - t / (s tau).  stats (R, 4): m, 1 / s, -t / (s tau), unused: what the
+// backward needs.  logp64 (R): the log-probability unrounded, for the sums of the preference loss.
+struct LogprobOut {
+    float* logp;
+    float* entropy;
+    float4* stats;
+    double* logp64;
+};
+
+template <typename E, int NT>
+__global__ __launch_bounds__(NT) void logprob_kernel(Rows rows, double inv_tau, LogprobOut out)
+{
+    __shared__ float sh[16];
+    const int64_t r = blockIdx.x;
+    if (!rows.kept(r)) {
+        if (threadIdx.x == 0) {
+            if (out.logp) out.logp[r] = 0.f;
+            if (out.entropy) out.entropy[r] = 0.f;
+            if (out.logp64) out.logp64[r] = 0.0;
+        }
+        return;
+    }
+    const typename E::Store* x = reinterpret_cast<const typename E::Store*>(rows.x) + r * rows.ld;
+    Row<E, NT> row(x, rows.vocab);
+    row.load_single();
+    float m, s, t;
+    row_stats(row, (float)(LOG2E * inv_tau), m, s, t, sh);
+    if (threadIdx.x == 0) {
+        const int64_t y = rows.targets[r];
+        const double log_s = log((double)s), u = -(double)t / (double)s * inv_tau;
+        const double lp = (y >= 0 && y < rows.vocab) ? ((double)E::load(x + y) - (double)m) * inv_tau - log_s : __builtin_nan("");
+        if (out.logp) out.logp[r] = (float)lp;
+        if (out.entropy) out.entropy[r] = (float)(log_s + u);
+        if (out.logp64) out.logp64[r] = lp;
+        if (out.stats) out.stats[r] = make_float4(m, 1.f / s, (float)u, 0.f);
+    }
+}
+
+// d/dx_j = (1/tau) [ g_l (1[j = y] - p_j) - g_H p_j (log p_j + H) ],  log p_j + H = (x_j - m) / tau + u
+// The coefficients g_l are one per row, or one per sequence: group 0: g_l[r], S > 0: g_l[r mod S] (time-major),
+// S < 0: g_l[r / -S] (sequence by sequence).
+struct RowGrad {
+    const float4* stats;
+    const float* g_logp;
+    const float* g_entropy;  // nullable
+    const float* gscale;     // nullable, one number
+    const float* gloss;      // nullable, one number per pair of sequences: g_l times gloss[sequence mod (S / 2)]
+    int64_t group;
+    int64_t pairs;
+    double inv_tau;
+    void* dx;
+    int64_t ldg;
+};
+
+template <typename E, int NT>
+__global__ __launch_bounds__(NT) void logprob_bwd_kernel(Rows rows, RowGrad g)
+{
+    const int64_t r = blockIdx.x;
+    const typename E::Store* x = reinterpret_cast<const typename E::Store*>(rows.x) + r * rows.ld;
+    Row<E, NT> row(x, rows.vocab);
+    const OutRow<E> out(g.dx, g.ldg, r, x);
+    if (!rows.kept(r)) {
+        fill_row(row, out, 0.f);
+        return;
+    }
+    row.load_single();
+    const int64_t y64 = rows.targets[r];
+    const bool bad = y64 < 0 || y64 >= rows.vocab;
+    const int y = bad ? -1 : (int)y64;
+    const int64_t b = g.group == 0 ? r : (g.group > 0 ? r % g.group : r / -g.group);
+    float gl = g.g_logp ? g.g_logp[b] : 0.f;
+    if (g.gscale) gl *= *g.gscale;
+    if (g.gloss) gl *= g.gloss[b % g.pairs];
+    if (bad) gl = __builtin_nanf("");
+    const float4 st = g.stats[r];
+    const float gh = g.g_entropy ? g.g_entropy[r] : 0.f;
+    const float c = (float)(LOG2E * g.inv_tau), it = (float)g.inv_tau, m = st.x;
+    // exp(c (x - m)) (k0 + k1 (x - m)) + [j = y] gy
+    const float gy = gl * it, k0 = -(gl + gh * st.z) * it * st.y, k1 = -gh * it * it * st.y;
+    auto value = [&](int j, float xv) {
+        const float d = xv - m;
+        float v = exp2f(d * c) * (k0 + k1 * clamped(d));
+        return j == y ? v + gy : v;
+    };
+    row.each([&](int j, const u32x4& v) {
+        float f[E::VEC];
+#pragma unroll
+        for (int q = 0; q < E::VEC; ++q) f[q] = value(j + q, E::get(v, q));
+        out.vec(j, f);
+    });
+    if (row.je >= 0) out.one(row.je, value(row.je, row.xe));
+}
+
+// ---- clipped policy loss -------------------------------------------------------------------------------------------
+// rho = exp(logp - old), l = -min(rho A, clip(rho, lo, hi) A) + kl (exp(ref - logp) - (ref - logp) - 1) - ent H
+// dl/dlogp = -[rho A <= clip(rho) A] rho A + kl (1 - exp(ref - logp)),  dl/dH = -ent
+struct Policy {
+    const float* old_logp;
+    const float* adv;
+    int64_t adv_rows;         // adv[r mod adv_rows]
+    const float* ref_logp;    // nullable
+    double lo, hi, kl, ent, inv_tau;
+    Weight w;
+    int skip_unit;            // nothing is done where *w.gscale is 1
+    float* row_loss;          // nullable, as the next two
+    float* logp;
+    float* entropy;
+    void* dx;                 // nullable
+    int64_t ldg;
+};
+
+template <typename E, int NT>
+__global__ __launch_bounds__(NT) void policy_kernel(Rows rows, Policy a)
+{
+    __shared__ float sh[16];
+    __shared__ float coef[3];
+    if (a.skip_unit && *a.w.gscale == 1.f) return;
+    const int64_t r = blockIdx.x;
+    const typename E::Store* x = reinterpret_cast<const typename E::Store*>(rows.x) + r * rows.ld;
+    Row<E, NT> row(x, rows.vocab);
+    const OutRow<E> out(a.dx, a.ldg, r, x);
+    if (!rows.kept(r)) {
+        if (threadIdx.x == 0) {
+            if (a.row_loss) a.row_loss[r] = 0.f;
+            if (a.logp) a.logp[r] = 0.f;
+            if (a.entropy) a.entropy[r] = 0.f;
+        }
+        if (a.dx) fill_row(row, out, 0.f);
+        return;
+    }
+    row.load_single();
+    float m, s, t;
+    const float c = (float)(LOG2E * a.inv_tau);
+    row_stats(row, c, m, s, t, sh);
+    const int64_t y64 = rows.targets[r];
+    const int y = (y64 >= 0 && y64 < rows.vocab) ? (int)y64 : -1;
+    if (threadIdx.x == 0) {
+        const double it = a.inv_tau, log_s = log((double)s), u = -(double)t / (double)s * it, H = log_s + u;
+        const double lp = y >= 0 ? ((double)E::load(x + y) - (double)m) * it - log_s : __builtin_nan("");
+        const double A = (double)a.adv[r % a.adv_rows];
+        const double rho = exp(lp - (double)a.old_logp[r]);
+        const double free = rho * A, held = (rho < a.lo ? a.lo : rho > a.hi ? a.hi : rho) * A;
+        double loss = free <= held ? -free : -held, g = free <= held ? -free : 0.0;
+        if (free != free) loss = g = free;  // a NaN stays one
+        if (a.ref_logp) {
+            const double gap = (double)a.ref_logp[r] - lp, away = exp(gap);
+            loss += a.kl * (away - gap - 1.0);
+            g += a.kl * (1.0 - away);
+        }
+        if (a.ent != 0.0) loss -= a.ent * H;
+        if (a.row_loss) a.row_loss[r] = (float)loss;
+        if (a.logp) a.logp[r] = (float)lp;
+        if (a.entropy) a.entropy[r] = (float)H;
+        if (a.dx) {
+            const double w = a.w.of(r) * it;
+            coef[0] = (float)(w * (-g + a.ent * u) / (double)s);
+            coef[1] = (float)(w * a.ent * it / (double)s);
+            coef[2] = (float)(w * g);
+        }
+    }
+    if (!a.dx) return;
+    __syncthreads();
+    const float k0 = coef[0], k1 = coef[1], gy = coef[2];
+    auto value = [&](int j, float xv) {
+        const float d = xv - m;
+        float v = exp2f(d * c) * (k0 + k1 * clamped(d));
+        return j == y ? v + gy : v;
+    };
+    row.each([&](int j, const u32x4& v) {
+        float f[E::VEC];
+#pragma unroll
+        for (int q = 0; q < E::VEC; ++q) f[q] = value(j + q, E::get(v, q));
+        out.vec(j, f);
+    });
+    if (row.je >= 0) out.one(row.je, value(row.je, row.xe));
+}
+
+// ---- distillation from a teacher's list of logits ----------------------------------------------------------------
+// The teacher gives k classes with logits t_k, and the log mass `tail` of all others at the same temperature; q is the
+// soft-max over the k + 1 of them.  The student's p is summed the same way: p_k, and p_t over the classes not listed.
+//   l = (1 - a) tau^2 [ sum q_k log(q_k / p_k) + q_t log(q_t / p_t) ] + a CE(y)
+//   dl/dx_j = (1 - a) tau (p_j - q_j)            for a listed class
+//           = (1 - a) tau p_j (1 - q_t / p_t)    for the others          plus a (softmax(x)_j - 1[j = y])
+// p_t is the sum of the others' own exponentials relative to their own maximum, not one minus the listed ones': it keeps
+// its relative precision however little is left.  The listed classes are marked in a bit map over the row (LDS) and
+// taken out of the sweeps; their gradients are stored after the row's.  A class listed twice is one class of the
+// student's (counted once in p) with the sum of its q.
+constexpr int DISTILL_MAX_K = 256;
+constexpr int DISTILL_MAX_VOCAB = 400000;  // bit map of 50 KB
+
+struct Distill {
+    const void* values;
+    int value_type;
+    const int32_t* indices;
+    int k;
+    const float* tail;   // nullable
+    double inv_tau, tau, ce;
+    Weight w;
+    int skip_unit;
+    float* row_loss;     // nullable
+    void* dx;            // nullable
+    int64_t ldg;
+};
+
+__device__ __forceinline__ float load_as(const void* p, int type, int64_t i)
+{
+    if (type == GTG_DTYPE_F32) return reinterpret_cast<const float*>(p)[i];
+    if (type == GTG_DTYPE_F16) return (float)reinterpret_cast<const _Float16*>(p)[i];
+    return (float)reinterpret_cast<const __bf16*>(p)[i];
+}
+
+template <typename E, int NT, bool TWO>
+__global__ __launch_bounds__(NT) void distill_kernel(Rows rows, Distill a)
+{
+    extern __shared__ unsigned bits[];  // (vocab + 31) / 32
+    __shared__ float sh[16];
+    __shared__ int sidx[DISTILL_MAX_K];    // class, -1 where the entry takes no part
+    __shared__ float st[DISTILL_MAX_K], sx[DISTILL_MAX_K], sq[DISTILL_MAX_K];
+    __shared__ unsigned char own[DISTILL_MAX_K];
+    __shared__ int bad, twice;
+    __shared__ float coef[3];  // of exp((x - m_t) / tau), of exp(x - m_t), of the target
+    __shared__ double glob[6];
+
+    if (a.skip_unit && *a.w.gscale == 1.f) return;
+    const int64_t r = blockIdx.x;
+    const typename E::Store* x = reinterpret_cast<const typename E::Store*>(rows.x) + r * rows.ld;
+    Row<E, NT> row(x, rows.vocab);
+    const OutRow<E> out(a.dx, a.ldg, r, x);
+    if (!rows.kept(r)) {
+        if (threadIdx.x == 0 && a.row_loss) a.row_loss[r] = 0.f;
+        if (a.dx) fill_row(row, out, 0.f);
+        return;
+    }
+    const int tid = threadIdx.x;
+    const int64_t y64 = rows.targets[r];
+    const int y = (y64 >= 0 && y64 < rows.vocab) ? (int)y64 : -1;
+    for (int i = tid; i < (rows.vocab + 31) / 32; i += NT) bits[i] = 0;
+    if (tid == 0) {
+        bad = y < 0;
+        twice = 0;
+    }
+    __syncthreads();
+    for (int k = tid; k < a.k; k += NT) {
+        const int j = a.indices[r * a.k + k];
+        const bool in = j >= 0 && j < rows.vocab;
+        if (j >= rows.vocab) bad = 1;  // (every writer writes the same value)
+        sidx[k] = in ? j : -1;
+        st[k] = in ? load_as(a.values, a.value_type, r * a.k + k) : neg_inf();
+        sx[k] = in ? E::load(x + j) : neg_inf();
+        own[k] = in;
+        if (in && (atomicOr(&bits[j >> 5], 1u << (j & 31)) >> (j & 31) & 1) != 0) twice = 1;
+    }
+    row.load_single();
+    __syncthreads();
+    if (twice) {  // of a class listed more than once the first entry stands for all: in a fixed order, so sums repeat
+        for (int k = tid; k < a.k; k += NT)
+            for (int i = 0; i < k; ++i)
+                if (sidx[i] == sidx[k]) own[k] = 0;
+        __syncthreads();
+    }
+    auto listed = [&](int j) { return (bits[j >> 5] >> (j & 31) & 1) != 0; };
+    const float xe = row.je >= 0 && !listed(row.je) ? row.xe : neg_inf();
+
+    // the classes outside the list: maximum, sums at both temperatures
+    float mx = xe;
+    row.each([&](int j, const u32x4& v) {
+#pragma unroll
+        for (int q = 0; q < E::VEC; ++q) mx = fmaxf(mx, listed(j + q) ? neg_inf() : E::get(v, q));
+    });
+    const float m_rest = block_max<NT>(mx, sh);
+    const float mt = finite_or_zero(m_rest);
+    const float c = (float)(LOG2E * a.inv_tau), c1 = (float)LOG2E;
+    float s_tau = 0.f, s_one = 0.f;
+    auto add = [&](float xv) {
+        const float d = xv - mt;
+        s_tau += exp2f(d * c);
+        if (TWO) s_one += exp2f(d * c1);
+    };
+    add(xe);
+    row.each([&](int j, const u32x4& v) {
+#pragma unroll
+        for (int q = 0; q < E::VEC; ++q) add(listed(j + q) ? neg_inf() : E::get(v, q));
+    });
+    s_tau = block_sum<NT>(s_tau, sh);
+    s_one = TWO ? block_sum<NT>(s_one, sh) : s_tau;
+
+    // one wave: the teacher's distribution, the student's sums over everything, the loss
+    if (tid < 64) {
+        const double it = a.inv_tau;
+        const double tail = a.tail ? (double)a.tail[r] : -(double)__builtin_inff();
+        float tm = neg_inf(), xm = m_rest;
+        for (int k = tid; k < a.k; k += 64) {
+            tm = fmaxf(tm, st[k]);
+            if (own[k]) xm = fmaxf(xm, sx[k]);
+        }
+        tm = wave_max(tm);
+        xm = wave_max(xm);
+        const double M0 = fmax((double)tm * it, tail), M = M0 > -1e300 ? M0 : 0.0;  // an infinite one would leave NaN in every difference
+        const float m = finite_or_zero(xm);
+        double z = 0.0, s = 0.0, s1 = 0.0, cross = 0.0;
+        for (int k = tid; k < a.k; k += 64) {
+            const double u = (double)st[k] * it;
+            const float q = exp2f((float)((u - M) * LOG2E));
+            sq[k] = q;
+            z += (double)q;
+            if (q != 0.f) cross += (double)q * ((u - M) - ((double)sx[k] - (double)m) * it);
+            if (own[k]) {
+                s += (double)exp2f((sx[k] - m) * c);
+                if (TWO) s1 += (double)exp2f((sx[k] - m) * c1);
+            }
+        }
+        z = wave_sum(z);
+        s = wave_sum(s);
+        s1 = TWO ? wave_sum(s1) : 0.0;
+        cross = wave_sum(cross);
+        const double qt0 = tail > -1e300 || tail != tail ? exp(tail - M) : 0.0;
+        z += qt0;
+        // exp of (the others' maximum) - (the row's): in 64 bits, for it scales every class outside the list
+        const double gap = (double)m_rest - (double)m;
+        const double lift = exp(gap * it), lift1 = TWO ? exp(gap) : lift;
+        s += (double)s_tau * lift;
+        s1 = TWO ? s1 + (double)s_one * lift1 : s;
+        const bool none = z == 0.0;  // the teacher says nothing about this row
+        const double qt = none ? 0.0 : qt0 / z;
+        double kd = 0.0;
+        const double wkd = 1.0 - a.ce;
+        if (!none && wkd != 0.0) {
+            // everything relative to the two maxima M and m, which may be as large as the type's lowest value
+            kd = cross / z - (log(z) - log(s));
+            if (qt != 0.0) kd += qt * ((tail - M) - (log((double)s_tau) + gap * it));
+            kd *= wkd * a.tau * a.tau;
+        }
+        double ce = 0.0;
+        if (a.ce != 0.0 && y >= 0) ce = a.ce * (log(s1) - ((double)E::load(x + y) - (double)m));
+        if (tid == 0) {
+            double loss = kd + ce;
+            if (bad) loss = __builtin_nan("");
+            if (a.row_loss) a.row_loss[r] = (float)loss;
+            const double w = bad ? __builtin_nan("") : a.w.of(r);
+            const double wk = none || wkd == 0.0 ? 0.0 : w * wkd * a.tau, wc = w * a.ce;
+            const double ka = wk == 0.0 ? 0.0 : wk * (lift / s - (qt != 0.0 ? qt / (double)s_tau : 0.0)), kb = wc * lift1 / s1;
+            coef[0] = (float)(TWO ? ka : ka + kb);
+            coef[1] = (float)kb;
+            coef[2] = (float)wc;
+            glob[0] = wk / s;                   // of exp((x_k - m) / tau)
+            glob[1] = none ? 0.0 : wk / z;      // of q_k
+            glob[2] = wc / s1;                  // of exp(x_k - m)
+            glob[3] = (double)m;
+        }
+    }
+    if (!a.dx) return;
+    __syncthreads();
+    const float ka = coef[0], kb = coef[1], gy = coef[2];
+    auto value = [&](int j, float xv) {
+        const float d = xv - mt;
+        float v = exp2f(d * c) * ka;
+        if (TWO) v += exp2f(d * c1) * kb;
+        return j == y ? v - gy : v;
+    };
+    row.each([&](int j, const u32x4& v) {
+        float f[E::VEC];
+#pragma unroll
+        for (int q = 0; q < E::VEC; ++q) f[q] = value(j + q, E::get(v, q));
+        out.vec(j, f);
+    });
+    if (row.je >= 0) out.one(row.je, value(row.je, row.xe));
+    __syncthreads();  // the listed classes' gradients go over what the row's vectors left in their places
+    for (int k = tid; k < a.k; k += NT) {
+        if (!own[k]) continue;
+        float q = sq[k];
+        if (twice)
+            for (int i = k + 1; i < a.k; ++i)
+                if (sidx[i] == sidx[k]) q += sq[i];
+        const float d = sx[k] - (float)glob[3];
+        double v = (double)exp2f(d * c) * glob[0] - (double)q * glob[1];
+        if (a.ce != 0.0) v += (double)exp2f(d * c1) * glob[2];
+        if (sidx[k] == y) v -= (double)gy;
+        out.one(sidx[k], (float)v);
+    }
+}
+
+// ---- the k largest logits of a row --------------------------------------------------------------------------------
+// Exact: larger first, equal ones by ascending index (-0 equals +0, a NaN is larger than every number).  The k-th
+// largest is found bit by bit on integers in the order of the values, ties by bits of the index.
+constexpr int TOP_MAX_K = 256;
+
+__device__ __forceinline__ unsigned order_key(float x)
+{
+    const unsigned b = __float_as_uint(x + 0.f);
+    return x != x ? 0xffffffffu : (b & 0x80000000u) ? ~b : b | 0x80000000u;
+}
+
+template <typename E, int NT>
+__global__ __launch_bounds__(NT) void top_kernel(const void* logits, int64_t ld, int V, int k, double inv_tau,
+                                                 void* __restrict__ values, int32_t* __restrict__ indices,
+                                                 float* __restrict__ tail)
+{
+    __shared__ float shf[16];
+    __shared__ int sh[16];
+    __shared__ int fill;
+    __shared__ unsigned ckey[TOP_MAX_K];
+    __shared__ int cidx[TOP_MAX_K];
+    const int64_t r = blockIdx.x;
+    const int tid = threadIdx.x;
+    const typename E::Store* x = reinterpret_cast<const typename E::Store*>(logits) + r * ld;
+    Row<E, NT> row(x, V);
+    row.load_single();
+    auto count = [&](auto pred) {
+        int n = row.je >= 0 && pred(row.je, row.xe) ? 1 : 0;
+        row.each([&](int j, const u32x4& v) {
+#pragma unroll
+            for (int q = 0; q < E::VEC; ++q) n += pred(j + q, E::get(v, q)) ? 1 : 0;
+        });
+        return block_count<NT>(n, sh);
+    };
+    unsigned kth = 0;  // the largest key that at least k elements reach
+    for (int bit = 31; bit >= 0; --bit) {
+        const unsigned cand = kth | (1u << bit);
+        if (count([&](int, float v) { return order_key(v) >= cand; }) >= k) kth = cand;
+    }
+    const int need = k - count([&](int, float v) { return order_key(v) > kth; });
+    int last = 0;  // the need-th element of that key, by index
+    for (int bit = 30; bit >= 0; --bit) {
+        const int cand = last + (1 << bit);
+        if (cand < V && count([&](int j, float v) { return j < cand && order_key(v) == kth; }) < need) last = cand;
+    }
+    auto chosen = [&](int j, float v) {
+        const unsigned key = order_key(v);
+        return key > kth || (key == kth && j <= last);
+    };
+    if (tid == 0) fill = 0;
+    __syncthreads();
+    auto take = [&](int j, float v) {
+        if (chosen(j, v)) {
+            const int at = atomicAdd(&fill, 1);
+            ckey[at] = order_key(v);
+            cidx[at] = j;
+        }
+    };
+    if (row.je >= 0) take(row.je, row.xe);
+    float mx = row.je >= 0 && !chosen(row.je, row.xe) ? row.xe : neg_inf();
+    row.each([&](int j, const u32x4& v) {
+#pragma unroll
+        for (int q = 0; q < E::VEC; ++q) {
+            const float f = E::get(v, q);
+            take(j + q, f);
+            if (!chosen(j + q, f)) mx = fmaxf(mx, f);
+        }
+    });
+    const float m_rest = block_max<NT>(mx, shf);  // (its barriers also close the list)
+    const float m = finite_or_zero(m_rest);
+    float s = 0.f;
+    const float c = (float)(LOG2E * inv_tau);
+    if (row.je >= 0 && !chosen(row.je, row.xe)) s += exp2f((row.xe - m) * c);
+    row.each([&](int j, const u32x4& v) {
+#pragma unroll
+        for (int q = 0; q < E::VEC; ++q) {
+            const float f = E::get(v, q);
+            if (!chosen(j + q, f)) s += exp2f((f - m) * c);
+        }
+    });
+    s = block_sum<NT>(s, shf);
+    if (tid == 0) tail[r] = m_rest == __builtin_inff() && s != s ? m_rest : (float)(log((double)s) + (double)m * inv_tau);
+    __syncthreads();
+    for (int i = tid; i < k; i += NT) {
+        int rank = 0;
+        for (int o = 0; o < k; ++o) rank += ckey[o] > ckey[i] || (ckey[o] == ckey[i] && cidx[o] < cidx[i]) ? 1 : 0;
+        indices[r * k + rank] = cidx[i];
+        reinterpret_cast<typename E::Store*>(values)[r * k + rank] = x[cidx[i]];
+    }
+}
+
+// ---- preference loss over pairs of sequences -------------------------------------------------------------------------
+// seq_b = sum over time of logp, margin = beta ((seq_c - ref_c) - (seq_r - ref_r)),
+// l = -(1 - e) log sigma(margin) - e log sigma(-margin);  the first `pairs` sequences are the chosen ones, sequence
+// b + pairs is the one rejected for b.  One block: sums in 64 bits and in a fixed order.
+struct Prefer {
+    const double* logp;   // (rows)
+    double* seq;          // (2 pairs) scratch
+    int64_t T, pairs;
+    int batch_first;
+    const float* ref;     // (2 pairs)
+    double beta, eps;
+    int mean;
+    float* seq_logp;      // (2 pairs)
+    float* coef;          // (2 pairs): dl / dseq
+    float* pair_loss;     // (pairs)
+    float* loss;          // nullable
+};
+
+__global__ __launch_bounds__(1024) void prefer_kernel(Prefer a)
+{
+    __shared__ double part[1024];
+    const int64_t S = 2 * a.pairs;
+    // G threads per sequence, neighbours on neighbouring sequences
+    const int width = (int)(S < 1024 ? S : 1024), G = 1024 / width;
+    const int lane = threadIdx.x % width, g = threadIdx.x / width;
+    for (int64_t b0 = 0; b0 < S; b0 += width) {
+        const int64_t b = b0 + lane;
+        double s = 0.0;
+        if (b < S && g < G)
+            for (int64_t t = g; t < a.T; t += G) s += a.logp[a.batch_first ? b * a.T + t : t * S + b];
+        part[threadIdx.x] = s;
+        __syncthreads();
+        if (g == 0 && b < S) {
+            for (int i = 1; i < G; ++i) s += part[i * width + lane];
+            a.seq[b] = s;
+            a.seq_logp[b] = (float)s;
+        }
+        __syncthreads();
+    }
+    double total = 0.0;
+    for (int64_t p = threadIdx.x; p < a.pairs; p += 1024) {
+        const double mg = a.beta * ((a.seq[p] - (double)a.ref[p]) - (a.seq[p + a.pairs] - (double)a.ref[p + a.pairs]));
+        const double both = log1p(exp(-fabs(mg)));
+        double l = (1.0 - a.eps) * (both + (mg < 0.0 ? -mg : 0.0));
+        if (a.eps != 0.0) l += a.eps * (both + (mg > 0.0 ? mg : 0.0));
+        const double dm = (a.eps - 1.0 / (1.0 + exp(mg))) * a.beta / (a.mean ? (double)a.pairs : 1.0);
+        a.pair_loss[p] = (float)l;
+        a.coef[p] = (float)dm;
+        a.coef[p + a.pairs] = (float)-dm;
+        total += l;
+    }
+    if (!a.loss) return;
+    part[threadIdx.x] = total;
+    __syncthreads();
+    if (threadIdx.x < 64) {
+        total = 0.0;
+        for (int i = 0; i < 16; ++i) total += part[threadIdx.x + 64 * i];
+        total = wave_sum(total);
+        if (threadIdx.x == 0) *a.loss = (float)(a.mean ? total / (double)a.pairs : total);
+    }
+}
+
+// A block per row: as many threads as the row's vectors keep busy.
+#define GTG_BY_SIZE(DTYPE, VOCAB, CALL)                                  \
+    do {                                                                 \
+        const int64_t bytes_ = (int64_t)(VOCAB) * ((DTYPE) == GTG_DTYPE_F32 ? 4 : 2); \
+        if ((DTYPE) == GTG_DTYPE_F32) {                                  \
+            typedef F32 E;                                               \
+            if (bytes_ <= 4096) { constexpr int NT = 64; CALL; }         \
+            else if (bytes_ <= 32768) { constexpr int NT = 256; CALL; }  \
+            else { constexpr int NT = 512; CALL; }                       \
+        } else if ((DTYPE) == GTG_DTYPE_F16) {                           \
+            typedef F16 E;                                               \
+            if (bytes_ <= 4096) { constexpr int NT = 64; CALL; }         \
+            else if (bytes_ <= 32768) { constexpr int NT = 256; CALL; }  \
+            else { constexpr int NT = 512; CALL; }                       \
+        } else {                                                         \
+            typedef BF16 E;                                              \
+            if (bytes_ <= 4096) { constexpr int NT = 64; CALL; }         \
+            else if (bytes_ <= 32768) { constexpr int NT = 256; CALL; }  \
+            else { constexpr int NT = 512; CALL; }                       \
+        }                                                                \
+    } while (0)
+
+Rows as_rows(const TokenRows& t) { return Rows{t.logits, t.ld, t.vocab, t.targets, t.padidx, t.mask}; }
+
+}  // namespace
+
+int top_logits(const void* logits, int dtype, int64_t R, int V, int64_t ld, int k, double temperature, void* values,
+               int32_t* indices, float* tail, hipStream_t s)
+{
+    ProfScope prof(s, "top_logits", R, V, k);
+    const double it = 1.0 / temperature;
+    GTG_BY_SIZE(dtype, V, hipLaunchKernelGGL(HIP_KERNEL_NAME(top_kernel<E, NT>), dim3((unsigned)R), dim3(NT), 0, s, logits, ld, V,
+                                             k, it, values, indices, tail));
+    return check_launch("top_kernel");
+}
+
+int token_logprob_fwd(const TokenRows& t, double temperature, float* logp, float* entropy, float* stats, double* logp64,
+                      hipStream_t s)
+{
+    ProfScope prof(s, "token_logprob_fwd", t.rows, t.vocab, 0);
+    const LogprobOut out{logp, entropy, reinterpret_cast<float4*>(stats), logp64};
+    const double it = 1.0 / temperature;
+    GTG_BY_SIZE(t.dtype, t.vocab, hipLaunchKernelGGL(HIP_KERNEL_NAME(logprob_kernel<E, NT>), dim3((unsigned)t.rows), dim3(NT), 0,
+                                                     s, as_rows(t), it, out));
+    return check_launch("logprob_kernel");
+}
+
+int token_logprob_bwd(const TokenRows& t, double temperature, const float* stats, const float* g_logp, const float* g_entropy,
+                      const float* gscale, const float* gloss, int64_t group, int64_t pairs, void* dx, int64_t ldg,
+                      hipStream_t s)
+{
+    ProfScope prof(s, "token_logprob_bwd", t.rows, t.vocab, 0);
+    const RowGrad g{reinterpret_cast<const float4*>(stats), g_logp, g_entropy, gscale, gloss, group, pairs, 1.0 / temperature, dx, ldg};
+    GTG_BY_SIZE(t.dtype, t.vocab, hipLaunchKernelGGL(HIP_KERNEL_NAME(logprob_bwd_kernel<E, NT>), dim3((unsigned)t.rows), dim3(NT),
+                                                     0, s, as_rows(t), g));
+    return check_launch("logprob_bwd_kernel");
+}
+
+int count_rows(const TokenRows& t, double* norm, hipStream_t s)
+{
+    hipLaunchKernelGGL(count_kernel, dim3(1), dim3(1024), 0, s, as_rows(t), t.rows, norm);
+    return check_launch("count_kernel");
+}
+
+int total_loss(const float* row_loss, int64_t R, const double* norm, float* loss, hipStream_t s)
+{
+    hipLaunchKernelGGL(total_kernel, dim3(1), dim3(1024), 0, s, row_loss, R, norm, loss);
+    return check_launch("total_kernel");
+}
+
+int policy_rows(const TokenRows& t, const PolicyRows& p, const float* gloss, const float* gscale, const double* norm,
+                bool skip_unit, float* row_loss, float* logp, float* entropy, void* dx, int64_t ldg, hipStream_t s)
+{
+    ProfScope prof(s, "policy_rows", t.rows, t.vocab, dx != nullptr);
+    const Policy a{p.old_logp, p.advantages, p.adv_rows, p.ref_logp, 1.0 - p.clip_low, 1.0 + p.clip_high, p.kl_coef, p.entropy_coef,
+                   1.0 / p.temperature, Weight{gloss, gscale, norm}, skip_unit ? 1 : 0, row_loss, logp, entropy, dx, ldg};
+    GTG_BY_SIZE(t.dtype, t.vocab, hipLaunchKernelGGL(HIP_KERNEL_NAME(policy_kernel<E, NT>), dim3((unsigned)t.rows), dim3(NT), 0, s,
+                                                     as_rows(t), a));
+    return check_launch("policy_kernel");
+}
+
+int distill_max_vocab() { return DISTILL_MAX_VOCAB; }
+
+int distill_rows(const TokenRows& t, const DistillRows& d, const float* gloss, const float* gscale, const double* norm,
+                 bool skip_unit, float* row_loss, void* dx, int64_t ldg, hipStream_t s)
+{
+    ProfScope prof(s, "distill_rows", t.rows, t.vocab, dx != nullptr);
+    const Distill a{d.values, d.value_dtype, d.indices, d.k, d.tail, 1.0 / d.temperature, d.temperature, d.ce_weight,
+                    Weight{gloss, gscale, norm}, skip_unit ? 1 : 0, row_loss, dx, ldg};
+    const size_t lds = (size_t)((t.vocab + 31) / 32) * 4;
+    if (d.ce_weight != 0.0 && d.temperature != 1.0)
+        GTG_BY_SIZE(t.dtype, t.vocab, hipLaunchKernelGGL(HIP_KERNEL_NAME(distill_kernel<E, NT, true>), dim3((unsigned)t.rows), dim3(NT),
+                                                         lds, s, as_rows(t), a));
+    else
+        GTG_BY_SIZE(t.dtype, t.vocab, hipLaunchKernelGGL(HIP_KERNEL_NAME(distill_kernel<E, NT, false>), dim3((unsigned)t.rows), dim3(NT),
+                                                         lds, s, as_rows(t), a));
+    return check_launch("distill_kernel");
+}
+
+int prefer_pairs(const double* logp, double* seq, int64_t T, int64_t pairs, bool batch_first, const float* ref, double beta,
+                 double label_smoothing, bool mean, float* seq_logp, float* coef, float* pair_loss, float* loss, hipStream_t s)
+{
+    const Prefer a{logp, seq, T, pairs, batch_first ? 1 : 0, ref, beta, label_smoothing, mean ? 1 : 0, seq_logp, coef, pair_loss, loss};
+    hipLaunchKernelGGL(prefer_kernel, dim3(1), dim3(1024), 0, s, a);
+    return check_launch("prefer_kernel");
+}
+
+}  // namespace gtg

@@ -687,3 +687,363 @@ def dropout(x, p: float, training: bool = True):
     if not training or p <= 0.0:
         return x
     return DropoutFn.apply(x, float(p))
+
+
+# ---------------------------------------------------------------------------
+# losses and read-outs on rows of vocabulary logits
+# ---------------------------------------------------------------------------
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}   # GTG_DTYPE_*
+_REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}                      # GTG_REDUCE_*
+
+
+def _need(ok, msg):
+    if not ok:
+        raise _lib.GtgError(msg)
+
+
+def _token_rows(what, logits, targets):
+    """(logits as (rows, V) with unit stride along V, targets (rows) int64 contiguous): the tensors themselves where
+    their strides allow it, copies otherwise."""
+    _lib.require_cuda(logits, targets)
+    _need(logits.dtype in _DTYPES, f"{what}: logits must be float32, float16 or bfloat16, not {logits.dtype}")
+    _need(logits.dim() >= 1 and logits.shape[-1] >= 1, f"{what}: logits must be (..., vocab)")
+    x = logits if logits.dim() == 2 else logits.reshape(-1, logits.shape[-1])
+    if (x.stride(1) != 1 and x.shape[1] > 1) or (x.stride(0) < x.shape[1] and x.shape[0] > 1):
+        x = x.contiguous()
+    if targets is None:
+        return x, None
+    _need(targets.shape == logits.shape[:-1], f"{what}: targets {tuple(targets.shape)} do not match logits {tuple(logits.shape)}")
+    _same_device(what, x, targets)
+    _need(not (targets.is_floating_point() or targets.is_complex() or targets.dtype == torch.bool), f"{what}: targets must be integers")
+    if targets.dtype != torch.int64:
+        targets = targets.long()
+    return x, targets.contiguous()
+
+
+def _same_device(what, x, *others):
+    for t in others:
+        if t is not None and t.device != x.device:
+            raise _lib.GtgError(f"{what}: every tensor must be on the logits' device ({x.device}), not on {t.device}")
+
+
+def _row_floats(what, name, t, x, shape):
+    """A float tensor of the rows' shape as contiguous fp32 on the logits' device."""
+    _need(torch.is_tensor(t) and t.is_floating_point(), f"{what}: {name} must be a floating tensor")
+    _same_device(what, x, t)
+    _need(tuple(t.shape) == tuple(shape), f"{what}: {name} must be {tuple(shape)}, not {tuple(t.shape)}")
+    return _f32c(t.detach())
+
+
+def _mask_bytes(what, mask, x, shape):
+    if mask is None:
+        return None
+    _same_device(what, x, mask)
+    _need(tuple(mask.shape) == tuple(shape), f"{what}: mask must be {tuple(shape)}, not {tuple(mask.shape)}")
+    return (mask if mask.dtype == torch.bool else mask != 0).contiguous().view(torch.uint8)
+
+
+def _row_stride(x):
+    return x.stride(0) if x.shape[0] > 1 else max(x.stride(0), x.shape[1])
+
+
+def _grad_like(x):
+    """Uninitialised (rows, V) of x's type whose rows have x's rows' alignment modulo 16 bytes, so that the kernels
+    read and write whole 16-byte vectors; contiguous where x's rows allow that."""
+    R, V = x.shape
+    vec = 16 // x.element_size()
+    skew, off = (_row_stride(x) - V) % vec, x.data_ptr() % 16 // x.element_size()
+    if skew == 0 and off == 0:
+        return torch.empty((R, V), dtype=x.dtype, device=x.device)
+    buf = torch.empty((R * (V + skew) + vec,), dtype=x.dtype, device=x.device)
+    return buf[off:off + R * (V + skew)].view(R, V + skew)[:, :V]
+
+
+def _logits_args(x):
+    return x.data_ptr(), _DTYPES[x.dtype], x.shape[0], x.shape[1], _row_stride(x)
+
+
+def _float_arg(what, name, v):
+    _need(isinstance(v, (int, float)), f"{what}: {name} must be a number")
+    return float(v)
+
+
+def _opt(t):
+    return None if t is None else t.data_ptr()
+
+
+@_on_tensor_device
+def top_logits(logits, k: int, temperature: float = 1.0):
+    """A teacher's answer in short: the k largest logits of every row of (..., V) in descending order -- equal ones by
+    ascending index, a NaN above every number -- and the log mass of the rest.
+
+    Returns (values (..., k) of the logits' type, indices (..., k) int32, tail (...) fp32), tail = log sum exp(logits /
+    temperature) over the classes that were not selected (-inf where k == V).  1 <= k <= min(V, 256).  No gradient.
+    What ``distill_loss`` takes of a teacher."""
+    with torch.no_grad():
+        x, _ = _token_rows("top_logits", logits, None)
+        _need(isinstance(k, int) and 1 <= k <= min(256, x.shape[1]), "top_logits: k must be an integer in [1, min(vocab, 256)]")
+        lead = tuple(logits.shape[:-1])
+        values = torch.empty(lead + (k,), dtype=x.dtype, device=x.device)
+        indices = torch.empty(lead + (k,), dtype=torch.int32, device=x.device)
+        tail = torch.empty(lead, dtype=torch.float32, device=x.device)
+        check(_lib.lib().gtg_top_logits(*_logits_args(x), k, _float_arg("top_logits", "temperature", temperature),
+                                        values.data_ptr(), indices.data_ptr(), tail.data_ptr(), stream_ptr()), "gtg_top_logits")
+    return values, indices, tail
+
+
+class TokenLogprobFn(torch.autograd.Function):
+    """(log softmax(logits / temperature)[target], entropy of that distribution) per row, zeros where the target is
+    padidx; both differentiable.  The backward reads the logits once more and keeps four numbers per row."""
+
+    @staticmethod
+    @_on_tensor_device
+    def forward(ctx, logits, targets, padidx, temperature):
+        x, y = _token_rows("token_logprob", logits, targets)
+        temperature = _float_arg("token_logprob", "temperature", temperature)
+        logp = torch.empty(targets.shape, dtype=torch.float32, device=x.device)
+        entropy = torch.empty_like(logp)
+        stats = torch.empty((x.shape[0], 4), dtype=torch.float32, device=x.device) if ctx.needs_input_grad[0] else None
+        check(_lib.lib().gtg_token_logprob_fwd(*_logits_args(x), y.data_ptr(), int(padidx), temperature, logp.data_ptr(),
+                                               entropy.data_ptr(), _opt(stats), stream_ptr()), "gtg_token_logprob_fwd")
+        ctx.save_for_backward(x, y, stats)
+        ctx.key = (int(padidx), temperature, logits.shape)
+        ctx.set_materialize_grads(False)
+        return logp, entropy
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    @_on_tensor_device
+    def backward(ctx, g_logp, g_entropy):
+        x, y, stats = ctx.saved_tensors
+        padidx, temperature, shape = ctx.key
+        if g_logp is None and g_entropy is None:
+            return None, None, None, None
+        g_logp, g_entropy = _f32c(g_logp), _f32c(g_entropy)
+        dx = _grad_like(x)
+        check(_lib.lib().gtg_token_logprob_bwd(*_logits_args(x), y.data_ptr(), padidx, temperature, stats.data_ptr(),
+                                               _opt(g_logp), _opt(g_entropy), dx.data_ptr(), _row_stride(dx), stream_ptr()),
+              "gtg_token_logprob_bwd")
+        return dx.view(shape), None, None, None
+
+
+def token_logprob(logits, targets, padidx, temperature: float = 1.0):
+    """(logp, entropy), each of targets' shape: log softmax(logits / temperature) at the target and the entropy of that
+    distribution; logits (..., V) fp32, fp16 or bf16, targets (...) integers.  Rows whose target is padidx give zero, a
+    target outside the vocabulary NaN.  See TokenLogprobFn."""
+    return TokenLogprobFn.apply(logits, targets, padidx, temperature)
+
+
+class _RowLossFn(torch.autograd.Function):
+    """What the distillation and the policy loss share: a loss per row of logits and its gradient from one sweep.
+
+    With a scalar reduction and ``eager_grad`` the forward writes the logits' gradient for an upstream gradient of 1
+    along with the loss -- one read and one write of the logits' size in all -- and the backward hands that out: it
+    launches the gradient sweep again on condition that the upstream gradient, known on the device only, is not 1.
+    Without ``eager_grad``, and for reduction "none", the gradient is computed in the backward alone (two reads, one
+    write).  A second backward through a retained graph computes it anew."""
+
+    # subclasses: _prepare(ctx, logits, *args) -> (x, saved tensors, reduction, eager_grad); _fwd / _bwd: the library call
+    @classmethod
+    def _run_forward(cls, ctx, op, x, shape, lead, saved, reduction, eager_grad, extra_outputs=0):
+        _need(reduction in _REDUCTIONS, f"{op}: reduction must be one of {sorted(_REDUCTIONS)}")
+        scalar = reduction != "none"
+        dev = x.device
+        row_loss = torch.empty(lead, dtype=torch.float32, device=dev)
+        loss = torch.empty((), dtype=torch.float32, device=dev) if scalar else None
+        norm = torch.empty((1,), dtype=torch.float64, device=dev) if reduction == "mean" else None
+        dx = _grad_like(x) if scalar and eager_grad and ctx.needs_input_grad[0] else None
+        extra = [torch.empty(lead, dtype=torch.float32, device=dev) for _ in range(extra_outputs)]
+        L = _lib.lib()
+        check(getattr(L, f"gtg_{op}_fwd")(*_logits_args(x), *cls._args(saved, ctx.key), _REDUCTIONS[reduction], _opt(norm),
+                                          row_loss.data_ptr(), _opt(loss), *[t.data_ptr() for t in extra], _opt(dx),
+                                          x.shape[1] if dx is None else _row_stride(dx), stream_ptr()), f"gtg_{op}_fwd")
+        ctx.save_for_backward(x, norm, *saved)
+        ctx.dx, ctx.scalar, ctx.shape = dx, scalar, shape
+        return (loss if scalar else row_loss), extra
+
+    @classmethod
+    def _run_backward(cls, ctx, op, g):
+        x, norm, *saved = ctx.saved_tensors
+        g = _f32c(g)
+        dx, ctx.dx = ctx.dx, None          # handed out once: afterwards it is the receiver's
+        have = dx is not None
+        if not have:
+            dx = _grad_like(x)
+        check(getattr(_lib.lib(), f"gtg_{op}_bwd")(*_logits_args(x), *cls._args(saved, ctx.key), _opt(norm),
+                                                   None if ctx.scalar else g.data_ptr(), g.data_ptr() if ctx.scalar else None,
+                                                   int(have), dx.data_ptr(), _row_stride(dx), stream_ptr()), f"gtg_{op}_bwd")
+        return dx.view(ctx.shape)
+
+
+class DistillLossFn(_RowLossFn):
+    """Loss of a student's logits against the classes a teacher lists; see distill_loss."""
+
+    @staticmethod
+    def _args(saved, key):
+        y, values, indices, tail = saved
+        padidx, temperature, ce_weight = key
+        return (y.data_ptr(), padidx, values.data_ptr(), _DTYPES[values.dtype], indices.data_ptr(), values.shape[-1], _opt(tail),
+                temperature, ce_weight)
+
+    @staticmethod
+    @_on_tensor_device
+    def forward(ctx, logits, values, indices, targets, padidx, tail, temperature, ce_weight, reduction, eager_grad):
+        what = "distill_loss"
+        x, y = _token_rows(what, logits, targets)
+        lead = tuple(targets.shape)
+        _need(values.dtype in _DTYPES and values.dim() == len(lead) + 1 and tuple(values.shape[:-1]) == lead and
+              1 <= values.shape[-1] <= 256, f"{what}: values must be {lead + ('k',)}, k in [1, 256], float32, float16 or bfloat16")
+        _need(indices.dtype in (torch.int32, torch.int64) and indices.shape == values.shape,
+              f"{what}: indices must be int32 or int64 of values' shape")
+        _same_device(what, x, values, indices)
+        if indices.dtype == torch.int64:
+            # (what does not fit stays out of range, on its side)
+            indices = indices.clamp(-1, 2 ** 31 - 1).int()
+        values, indices = values.detach().contiguous(), indices.contiguous()
+        if tail is not None:
+            tail = _row_floats(what, "tail", tail, x, lead)
+        ctx.key = (int(padidx), _float_arg(what, "temperature", temperature), _float_arg(what, "ce_weight", ce_weight))
+        loss, _ = DistillLossFn._run_forward(ctx, what, x, logits.shape, lead, (y, values, indices, tail), reduction, eager_grad)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    @_on_tensor_device
+    def backward(ctx, g):
+        return (DistillLossFn._run_backward(ctx, "distill_loss", g),) + (None,) * 9
+
+
+def distill_loss(logits, values, indices, targets, padidx, tail=None, temperature: float = 1.0, ce_weight: float = 0.0,
+                 reduction: str = "mean", eager_grad: bool = True):
+    """Distillation of a teacher's top logits: per row
+
+        (1 - ce_weight) temperature^2 KL(q || p) + ce_weight (-log softmax(logits)[target])
+
+    q is the teacher's distribution over the k classes it lists -- values (..., k), indices (..., k), as ``top_logits``
+    gives them -- and, with ``tail`` (...), over "any other class", whose log mass at this temperature tail is; p is the
+    student's softmax(logits / temperature) over the same classes and the rest as one.  Without a tail the list is taken
+    for the teacher's whole distribution.  A negative index takes no part (a shorter list), one past the vocabulary gives
+    NaN; rows whose target is padidx take no part.
+
+    reduction: "mean" over the rows that count (0 if there are none), "sum", or "none" (a loss per row).  Differentiable
+    in the logits alone.  ``eager_grad=False`` for a scalar loss that will be scaled before its backward -- by a gradient
+    scaler, a number of accumulation steps -- : the gradient is then computed in the backward only, see _RowLossFn."""
+    return DistillLossFn.apply(logits, values, indices, targets, padidx, tail, temperature, ce_weight, reduction, eager_grad)
+
+
+class PolicyLossFn(_RowLossFn):
+    """Clipped policy loss with KL and entropy terms; see policy_loss."""
+
+    @staticmethod
+    def _args(saved, key):
+        y, old, adv, ref, mask = saved
+        padidx, scalars = key
+        return (y.data_ptr(), padidx, _opt(mask), old.data_ptr(), adv.data_ptr(), adv.numel(), _opt(ref)) + scalars
+
+    @staticmethod
+    @_on_tensor_device
+    def forward(ctx, logits, targets, padidx, old_logp, advantages, ref_logp, clip_low, clip_high, kl_coef, entropy_coef,
+                temperature, mask, reduction, eager_grad):
+        what = "policy_loss"
+        x, y = _token_rows(what, logits, targets)
+        lead = tuple(targets.shape)
+        old = _row_floats(what, "old_logp", old_logp, x, lead)
+        _need(torch.is_tensor(advantages), f"{what}: advantages must be a floating tensor")
+        per_column = len(lead) == 2 and tuple(advantages.shape) == lead[1:]
+        adv = _row_floats(what, "advantages", advantages, x, lead[1:] if per_column else lead)
+        ref = None if ref_logp is None else _row_floats(what, "ref_logp", ref_logp, x, lead)
+        scalars = tuple(_float_arg(what, n, v) for n, v in (("clip_low", clip_low), ("clip_high", clip_high), ("kl_coef", kl_coef),
+                                                            ("entropy_coef", entropy_coef), ("temperature", temperature)))
+        _need(scalars[2] == 0.0 or ref is not None, f"{what}: kl_coef needs ref_logp")
+        ctx.key = (int(padidx), scalars)
+        saved = (y, old, adv, ref, _mask_bytes(what, mask, x, lead))
+        loss, (logp, entropy) = PolicyLossFn._run_forward(ctx, what, x, logits.shape, lead, saved, reduction, eager_grad, 2)
+        ctx.mark_non_differentiable(logp, entropy)
+        ctx.set_materialize_grads(False)
+        return loss, logp, entropy
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    @_on_tensor_device
+    def backward(ctx, g, _glogp, _gentropy):
+        return (PolicyLossFn._run_backward(ctx, "policy_loss", g) if g is not None else None,) + (None,) * 13
+
+
+def policy_loss(logits, targets, padidx, old_logp, advantages, ref_logp=None, clip_low: float = 0.2, clip_high: float = 0.2,
+                kl_coef: float = 0.0, entropy_coef: float = 0.0, temperature: float = 1.0, mask=None, reduction: str = "mean",
+                eager_grad: bool = True):
+    """Clipped policy loss of sampled tokens.  Per row, with logp = log softmax(logits / temperature)[target] and rho =
+    exp(logp - old_logp):
+
+        -min(rho A, clip(rho, 1 - clip_low, 1 + clip_high) A) - entropy_coef entropy
+        + kl_coef (exp(ref_logp - logp) - (ref_logp - logp) - 1)
+
+    targets, old_logp, ref_logp, mask (...); advantages (...), or (B) for time-major (T, B) targets.  Rows whose target is
+    padidx or whose mask is false (a prompt's tokens) take no part.  Returns (loss, logp, entropy), the last two of
+    targets' shape and without gradient; reduction and eager_grad as in distill_loss.  Differentiable in the logits
+    alone."""
+    return PolicyLossFn.apply(logits, targets, padidx, old_logp, advantages, ref_logp, clip_low, clip_high, kl_coef, entropy_coef,
+                              temperature, mask, reduction, eager_grad)
+
+
+class PreferenceLossFn(torch.autograd.Function):
+    """Preference loss over pairs of sequences; see preference_loss.  The weight of every row's gradient depends on both
+    whole sequences, so the backward reads the logits once more."""
+
+    @staticmethod
+    @_on_tensor_device
+    def forward(ctx, logits, targets, padidx, ref_logp, beta, label_smoothing, mask, batch_first, reduction):
+        what = "preference_loss"
+        x, y = _token_rows(what, logits, targets)
+        _need(targets.dim() == 2, f"{what}: targets must be (T, 2 P), or (2 P, T) with batch_first")
+        _need(reduction in _REDUCTIONS, f"{what}: reduction must be one of {sorted(_REDUCTIONS)}")
+        S, T = targets.shape if batch_first else tuple(targets.shape)[::-1]
+        _need(S % 2 == 0, f"{what}: an even number of sequences is needed, the chosen ones first, then the rejected ones")
+        ref = _row_floats(what, "ref_logp", ref_logp, x, (S,))
+        m = _mask_bytes(what, mask, x, targets.shape)
+        beta, label_smoothing = _float_arg(what, "beta", beta), _float_arg(what, "label_smoothing", label_smoothing)
+        L, dev, P = _lib.lib(), x.device, S // 2
+        empty = lambda *shape: torch.empty(shape, dtype=torch.float32, device=dev)  # noqa: E731
+        stats, coef, seq_logp, pair_loss = empty(x.shape[0], 4), empty(S), empty(S), empty(P)
+        loss = empty() if reduction != "none" else None
+        ws = _ws(L.gtg_preference_workspace_bytes(T, P), dev)
+        ptr_x, dtype, _, V, ld = _logits_args(x)
+        ctx.head = (dtype, T, P, V, ld, int(bool(batch_first)))
+        check(L.gtg_preference_fwd(ptr_x, *ctx.head, y.data_ptr(), int(padidx), _opt(m), ref.data_ptr(), beta, label_smoothing,
+                                   _REDUCTIONS[reduction], stats.data_ptr(), coef.data_ptr(), seq_logp.data_ptr(),
+                                   pair_loss.data_ptr(), _opt(loss), ws.data_ptr(), ws.numel(), stream_ptr()), "gtg_preference_fwd")
+        ctx.save_for_backward(x, y, m, stats, coef)
+        ctx.padidx, ctx.scalar, ctx.shape = int(padidx), loss is not None, logits.shape
+        ctx.mark_non_differentiable(seq_logp)
+        ctx.set_materialize_grads(False)
+        return (pair_loss if loss is None else loss), seq_logp
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    @_on_tensor_device
+    def backward(ctx, g, _gseq):
+        if g is None:
+            return (None,) * 9
+        x, y, m, stats, coef = ctx.saved_tensors
+        g = _f32c(g)
+        dx = _grad_like(x)
+        check(_lib.lib().gtg_preference_bwd(x.data_ptr(), *ctx.head, y.data_ptr(), ctx.padidx, _opt(m), stats.data_ptr(),
+                                            coef.data_ptr(), g.data_ptr() if ctx.scalar else None,
+                                            None if ctx.scalar else g.data_ptr(), dx.data_ptr(), _row_stride(dx), stream_ptr()),
+              "gtg_preference_bwd")
+        return (dx.view(ctx.shape),) + (None,) * 8
+
+
+def preference_loss(logits, targets, padidx, ref_logp, beta: float = 0.1, label_smoothing: float = 0.0, mask=None,
+                    batch_first: bool = False, reduction: str = "mean"):
+    """Loss of preferred over rejected sequences.  logits (T, 2 P, V) and targets (T, 2 P), time-major as the decoder
+    gives them ((2 P, T, V) and (2 P, T) with batch_first): sequence b < P was chosen over sequence P + b.  With seq_logp the
+    sums of the tokens' log-probabilities over each sequence (targets equal to padidx, and tokens whose mask is false,
+    left out), ref_logp (2 P) the same sums under the reference model, and margin = beta ((seq_logp - ref_logp)[chosen] -
+    (seq_logp - ref_logp)[rejected]):
+
+        -(1 - label_smoothing) log sigma(margin) - label_smoothing log sigma(-margin)
+
+    Returns (loss, seq_logp (2 P), without gradient); reduction over the pairs: "mean", "sum" or "none".  Differentiable
+    in the logits alone."""
+    return PreferenceLossFn.apply(logits, targets, padidx, ref_logp, beta, label_smoothing, mask, batch_first, reduction)

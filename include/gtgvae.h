@@ -70,6 +70,15 @@ extern "C" {
 #define GTG_MATRIX_F16X2 2
 #define GTG_MATRIX_BF16X3 3
 
+/* Element types of the entry points that take logits. */
+#define GTG_DTYPE_F32 0
+#define GTG_DTYPE_F16 1
+#define GTG_DTYPE_BF16 2
+
+#define GTG_REDUCE_NONE 0
+#define GTG_REDUCE_SUM 1
+#define GTG_REDUCE_MEAN 2
+
 int gtg_version(void);
 const char* gtg_last_error(void);
 int gtg_max_nodes(void);
@@ -402,6 +411,91 @@ int gtg_embed_dropout_bwd(const float* dout, const int64_t* ids, int64_t rows, i
                           uint64_t seed, uint64_t stream_id, float* dtable, float* d_add, int add_rows, void* ws,
                           size_t ws_bytes, void* stream);
 int gtg_dropout(const float* x, int64_t count, float p, uint64_t seed, uint64_t stream_id, float* y, void* stream);
+
+/* ---- losses and read-outs on rows of vocabulary logits -----------------------
+ * No counterpart in the reference, whose only loss on the decoder's logits is the teacher-forced cross-entropy
+ * (src/text_vae.py:77-79): these are what a trained text decoder is distilled, scored and tuned with.
+ *
+ * Common to all of them
+ *   logits: `rows` rows of `vocab` elements of type `dtype` (GTG_DTYPE_*), row r at logits + r ld (ld >= vocab, in
+ *     elements; any alignment of a row that its elements allow).  In a time-major (T, B, vocab) tensor row t B + b.
+ *   targets (rows) int64: the row's token.  A row whose target equals padidx, or whose mask byte (rows, uint8,
+ *     nullable) is 0, is not read; its outputs, its loss and its gradient are zero.  A target outside [0, vocab) that
+ *     is not padidx gives NaN in the row's outputs and gradient.
+ *   temperature > 0: everything is a function of logits / temperature.
+ *   dlogits: the gradient, of the logits' type, row r at dlogits + r ldg, all `vocab` elements of every row written
+ *     (zeros where the row does not count); must not overlap the logits.  Stored fastest where a row's address modulo 16 is
+ *     that of its logits.
+ *   reduction: GTG_REDUCE_NONE (one loss per row or pair), _SUM, _MEAN (over the rows that count, or the pairs; 0
+ *     where there are none).
+ *   Sums over a row are held in 32 bits; logarithms, ratios and losses, one number per row, are computed in 64.
+ *   Masked logits of -inf or the type's lowest value count as such; a row of nothing but -inf, and a NaN or +inf
+ *   in a row, give NaN as the formulas do.
+ *
+ * gtg_top_logits: the k (1 <= k <= min(vocab, 256)) largest logits of every row in descending order, equal ones by
+ * ascending index, a NaN above every number: values (rows, k) of the logits' type, indices (rows, k) int32, and
+ * tail (rows): log sum exp(logits / temperature) over the classes not selected (-inf if there are none).
+ *
+ * gtg_token_logprob_fwd: logp (rows) = log softmax(logits / temperature)[target], entropy (rows) of that
+ * distribution, stats (rows, 4) for the backward.  _bwd: dlogits from g_logp and g_entropy (rows; either nullable).
+ *
+ * gtg_distill_loss_*: loss of a student's logits against the k classes a teacher lists per row, values (rows, k) of type
+ * value_dtype and indices (rows, k) int32 (negative: the entry takes no part; >= vocab: NaN), and tail (rows,
+ * nullable = -inf): the teacher's log mass of all other classes at the same temperature.  With q the soft-max of
+ * (values / temperature, tail) and p the student's softmax(logits / temperature) over the listed classes and the
+ * rest as one: (1 - ce_weight) temperature^2 KL(q || p) + ce_weight (-log softmax(logits)[target]).  Where the list says
+ * nothing (no entry, no tail) the first term is zero.  A class listed twice counts once in p.  vocab <= 400 000, k <= 256.
+ *
+ * gtg_policy_loss_*: with rho = exp(logp - old_logp), H the entropy and A = advantages[r mod adv_rows]:
+ *   -min(rho A, clip(rho, 1 - clip_low, 1 + clip_high) A) - entropy_coef H
+ *   + kl_coef (exp(ref_logp - logp) - (ref_logp - logp) - 1)                       (ref_logp nullable)
+ * logp, entropy (rows) are written along (nullable).
+ *
+ * For both: _fwd writes row_loss (rows) and, for _SUM and _MEAN, *loss and (for _MEAN) *norm, the factor of the mean; with
+ * dlogits not NULL it also writes the gradient of *loss (of the sum of row_loss for _NONE) in the same sweep over the
+ * logits.  _bwd writes the gradient alone, each row's weighted with gloss[r] (nullable), *gscale (nullable) and
+ * *norm (nullable).  With unless_unit != 0 it leaves dlogits as it is where *gscale is 1: for a caller that already has the
+ * gradient for 1 from _fwd and learns the scale only later, on the device.
+ *
+ * gtg_preference_*: 2 pairs sequences of T rows each (row t 2 pairs + b, or b T + t with batch_first); sequence b <
+ * pairs was chosen over sequence b + pairs.  seq_logp (2 pairs) = sum of logp over a sequence's rows, margin = beta
+ * ((seq - ref)[chosen] - (seq - ref)[rejected]) with ref_logp (2 pairs) the same sums under the reference model,
+ *   pair_loss (pairs) = -(1 - label_smoothing) log sigma(margin) - label_smoothing log sigma(-margin).
+ * stats (rows, 4) and coef (2 pairs) go to the backward, which takes gscale (one number, for _SUM and _MEAN) or gloss
+ * (pairs, for _NONE), both nullable.  ws: gtg_preference_workspace_bytes(). */
+int gtg_top_logits(const void* logits, int dtype, int64_t rows, int vocab, int64_t ld, int k, double temperature,
+                   void* values, int32_t* indices, float* tail, void* stream);
+int gtg_token_logprob_fwd(const void* logits, int dtype, int64_t rows, int vocab, int64_t ld, const int64_t* targets,
+                          int64_t padidx, double temperature, float* logp, float* entropy, float* stats, void* stream);
+int gtg_token_logprob_bwd(const void* logits, int dtype, int64_t rows, int vocab, int64_t ld, const int64_t* targets,
+                          int64_t padidx, double temperature, const float* stats, const float* g_logp,
+                          const float* g_entropy, void* dlogits, int64_t ldg, void* stream);
+int gtg_distill_loss_fwd(const void* logits, int dtype, int64_t rows, int vocab, int64_t ld, const int64_t* targets,
+                         int64_t padidx, const void* values, int value_dtype, const int32_t* indices, int k,
+                         const float* tail, double temperature, double ce_weight, int reduction, double* norm,
+                         float* row_loss, float* loss, void* dlogits, int64_t ldg, void* stream);
+int gtg_distill_loss_bwd(const void* logits, int dtype, int64_t rows, int vocab, int64_t ld, const int64_t* targets,
+                         int64_t padidx, const void* values, int value_dtype, const int32_t* indices, int k,
+                         const float* tail, double temperature, double ce_weight, const double* norm, const float* gloss,
+                         const float* gscale, int unless_unit, void* dlogits, int64_t ldg, void* stream);
+int gtg_policy_loss_fwd(const void* logits, int dtype, int64_t rows, int vocab, int64_t ld, const int64_t* targets,
+                        int64_t padidx, const uint8_t* mask, const float* old_logp, const float* advantages,
+                        int64_t adv_rows, const float* ref_logp, double clip_low, double clip_high, double kl_coef,
+                        double entropy_coef, double temperature, int reduction, double* norm, float* row_loss,
+                        float* loss, float* logp, float* entropy, void* dlogits, int64_t ldg, void* stream);
+int gtg_policy_loss_bwd(const void* logits, int dtype, int64_t rows, int vocab, int64_t ld, const int64_t* targets,
+                        int64_t padidx, const uint8_t* mask, const float* old_logp, const float* advantages,
+                        int64_t adv_rows, const float* ref_logp, double clip_low, double clip_high, double kl_coef,
+                        double entropy_coef, double temperature, const double* norm, const float* gloss,
+                        const float* gscale, int unless_unit, void* dlogits, int64_t ldg, void* stream);
+size_t gtg_preference_workspace_bytes(int64_t T, int64_t pairs);
+int gtg_preference_fwd(const void* logits, int dtype, int64_t T, int64_t pairs, int vocab, int64_t ld, int batch_first,
+                       const int64_t* targets, int64_t padidx, const uint8_t* mask, const float* ref_logp, double beta,
+                       double label_smoothing, int reduction, float* stats, float* coef, float* seq_logp, float* pair_loss,
+                       float* loss, void* ws, size_t ws_bytes, void* stream);
+int gtg_preference_bwd(const void* logits, int dtype, int64_t T, int64_t pairs, int vocab, int64_t ld, int batch_first,
+                       const int64_t* targets, int64_t padidx, const uint8_t* mask, const float* stats, const float* coef,
+                       const float* gscale, const float* gloss, void* dlogits, int64_t ldg, void* stream);
 
 /* ---- optimiser -------------------------------------------------------------
  * Replaces optim.Adam(lr, betas=(0.5, 0.999)).step() (src/train.py:290,314)
