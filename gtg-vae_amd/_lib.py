@@ -176,7 +176,8 @@ def ptr(t):
 def stream_ptr():
     import torch
 
-    return torch.cuda.current_stream().cuda_stream
+    # (the handle alone: building a torch.cuda.Stream around it costs 2.5 us per call)
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def require_cuda(*tensors):

@@ -1513,10 +1513,11 @@ int gtg_distill_loss_fwd(const void* logits, int dtype, int64_t rows, int vocab,
     hipStream_t s = (hipStream_t)stream;
     const TokenRows t{logits, dtype, rows, vocab, ld, targets, padidx, nullptr};
     if (reduction != GTG_REDUCE_MEAN) norm = nullptr;
-    if (norm) GTG_TRY(count_rows(t, norm, s));
+    const bool in_rows = norm && counts_in_rows(rows);
+    if (norm && !in_rows) GTG_TRY(count_rows(t, norm, s));
     if (rows > 0) {
         const DistillRows d{values, value_dtype, indices, k, tail, temperature, ce_weight};
-        GTG_TRY(distill_rows(t, d, nullptr, nullptr, norm, false, row_loss, dlogits, ldg, s));
+        GTG_TRY(distill_rows(t, d, nullptr, nullptr, norm, in_rows, false, row_loss, dlogits, ldg, s));
     }
     return reduction == GTG_REDUCE_NONE ? GTG_OK : total_loss(row_loss, rows, norm, loss, s);
 }
@@ -1535,7 +1536,7 @@ int gtg_distill_loss_bwd(const void* logits, int dtype, int64_t rows, int vocab,
     GTG_REQUIRE(targets != nullptr, "null pointer");
     const TokenRows t{logits, dtype, rows, vocab, ld, targets, padidx, nullptr};
     const DistillRows d{values, value_dtype, indices, k, tail, temperature, ce_weight};
-    return distill_rows(t, d, gloss, gscale, norm, unless_unit != 0, nullptr, dlogits, ldg, (hipStream_t)stream);
+    return distill_rows(t, d, gloss, gscale, const_cast<double*>(norm), false, unless_unit != 0, nullptr, dlogits, ldg, (hipStream_t)stream);
 }
 
 static const char* policy_fault(const PolicyRows& p, const int64_t* targets, int64_t rows)
@@ -1566,8 +1567,9 @@ int gtg_policy_loss_fwd(const void* logits, int dtype, int64_t rows, int vocab, 
     hipStream_t s = (hipStream_t)stream;
     const TokenRows t{logits, dtype, rows, vocab, ld, targets, padidx, mask};
     if (reduction != GTG_REDUCE_MEAN) norm = nullptr;
-    if (norm) GTG_TRY(count_rows(t, norm, s));
-    if (rows > 0) GTG_TRY(policy_rows(t, p, nullptr, nullptr, norm, false, row_loss, logp, entropy, dlogits, ldg, s));
+    const bool in_rows = norm && counts_in_rows(rows);
+    if (norm && !in_rows) GTG_TRY(count_rows(t, norm, s));
+    if (rows > 0) GTG_TRY(policy_rows(t, p, nullptr, nullptr, norm, in_rows, false, row_loss, logp, entropy, dlogits, ldg, s));
     return reduction == GTG_REDUCE_NONE ? GTG_OK : total_loss(row_loss, rows, norm, loss, s);
 }
 
@@ -1584,7 +1586,7 @@ int gtg_policy_loss_bwd(const void* logits, int dtype, int64_t rows, int vocab, 
     GTG_REQUIRE(!unless_unit || gscale, "unless_unit needs gscale");
     if (rows == 0) return GTG_OK;
     const TokenRows t{logits, dtype, rows, vocab, ld, targets, padidx, mask};
-    return policy_rows(t, p, gloss, gscale, norm, unless_unit != 0, nullptr, nullptr, nullptr, dlogits, ldg, (hipStream_t)stream);
+    return policy_rows(t, p, gloss, gscale, const_cast<double*>(norm), false, unless_unit != 0, nullptr, nullptr, nullptr, dlogits, ldg, (hipStream_t)stream);
 }
 
 size_t gtg_preference_workspace_bytes(int64_t T, int64_t pairs)

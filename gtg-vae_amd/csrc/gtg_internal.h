@@ -380,14 +380,16 @@ int token_logprob_fwd(const TokenRows& t, double temperature, float* logp, float
 int token_logprob_bwd(const TokenRows& t, double temperature, const float* stats, const float* g_logp, const float* g_entropy,
                       const float* gscale, const float* gloss, int64_t group, int64_t pairs, void* dx, int64_t ldg,
                       hipStream_t s);
-int count_rows(const TokenRows& t, double* norm, hipStream_t s);  // *norm = 1 / (rows that count), 0 if none
+// *norm = 1 / (rows that count), 0 if none; for few rows (counts_in_rows) the row kernels below do it themselves
+bool counts_in_rows(int64_t R);
+int count_rows(const TokenRows& t, double* norm, hipStream_t s);
 int total_loss(const float* row_loss, int64_t R, const double* norm, float* loss, hipStream_t s);
-// row r's gradient is weighted with gloss[r] * *gscale * *norm (each 1 where NULL); skip_unit: the launch does nothing
-// where *gscale is 1
-int policy_rows(const TokenRows& t, const PolicyRows& p, const float* gloss, const float* gscale, const double* norm,
+// row r's gradient is weighted with gloss[r] * *gscale * *norm (each 1 where NULL); count: *norm is found here;
+// skip_unit: the launch does nothing where *gscale is 1
+int policy_rows(const TokenRows& t, const PolicyRows& p, const float* gloss, const float* gscale, double* norm, bool count,
                 bool skip_unit, float* row_loss, float* logp, float* entropy, void* dx, int64_t ldg, hipStream_t s);
 int distill_max_vocab();
-int distill_rows(const TokenRows& t, const DistillRows& d, const float* gloss, const float* gscale, const double* norm,
+int distill_rows(const TokenRows& t, const DistillRows& d, const float* gloss, const float* gscale, double* norm, bool count,
                  bool skip_unit, float* row_loss, void* dx, int64_t ldg, hipStream_t s);
 int prefer_pairs(const double* logp, double* seq, int64_t T, int64_t pairs, bool batch_first, const float* ref, double beta,
                  double label_smoothing, bool mean, float* seq_logp, float* coef, float* pair_loss, float* loss,

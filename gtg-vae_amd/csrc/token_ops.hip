@@ -19,11 +19,15 @@ typedef _Float16 f16x2v __attribute__((ext_vector_type(2)));
 
 constexpr double LOG2E = 1.4426950408889634;
 __device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
+// The hardware's 2^x: 1 step off at most, 0 where the result would lie below 2^-126.  The library's exp2f spends five more
+// instructions on those, as much again as everything else done per logit.
+__device__ __forceinline__ float exp2_raw(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // 16 bytes of logits, element by element as fp32.
 struct F32 {
     typedef float Store;
     static constexpr int VEC = 4;
+    static constexpr unsigned NEG2 = 0xff800000u;  // -inf in every element of a dword
     __device__ static float get(const u32x4& v, int q) { return __uint_as_float(v[q]); }
     __device__ static void clear(u32x4& v, int q) { v[q] = 0xff800000u; }
     __device__ static float load(const Store* p) { return *p; }
@@ -39,6 +43,7 @@ struct F32 {
 struct BF16 {
     typedef __bf16 Store;
     static constexpr int VEC = 8;
+    static constexpr unsigned NEG2 = 0xff80ff80u;  // -inf in every element of a dword
     __device__ static float get(const u32x4& v, int q)
     {
         return __uint_as_float((q & 1) ? (v[q >> 1] & 0xffff0000u) : (v[q >> 1] << 16));
@@ -63,6 +68,7 @@ struct BF16 {
 struct F16 {
     typedef _Float16 Store;
     static constexpr int VEC = 8;
+    static constexpr unsigned NEG2 = 0xfc00fc00u;  // -inf in every element of a dword
     __device__ static float get(const u32x4& v, int q)
     {
         return (float)__builtin_bit_cast(_Float16, (unsigned short)((q & 1) ? (v[q >> 1] >> 16) : (v[q >> 1] & 0xffffu)));
@@ -89,32 +95,94 @@ struct F16 {
 // The row is cut where 16-byte alignment begins and ends: up to VEC - 1 elements in front and behind, taken one each by
 // the first 2 VEC threads (`xe`, `je`), and the body of whole vectors between them, vector i by thread i mod NT.  No
 // access leaves the row, whatever its alignment and length.
-template <typename E, int NT>
+// NV > 0: the body is loaded once into NV vectors of registers per thread (places past its end hold -inf) and every
+// sweep works on those: one read of the row.  NV == 0: every sweep reads the row again.
+// MARKED: classes marked in a bit map (LDS, Marks below) count as -inf: removed from the registers once, or as each vector is read.
+// Waves per SIMD that the kernels on NV vectors a thread are held to: enough blocks per CU to load one row while another is
+// summed or stored.
+constexpr int min_waves(int nv) { return nv == 16 ? 4 : nv == 8 ? 6 : 8; }
+template <typename E, int NT, int NV, bool MARKED = false>
 struct Row {
     typedef typename E::Store S;
     static constexpr int VEC = E::VEC;
     const S* p;
     int V, head, nb, je;  // elements in front, vectors in the body, this thread's single element or -1
     float xe;             // its value, -inf if there is none
+    const unsigned char* marks;
+    u32x4 v[NV > 0 ? NV : 1];
 
-    __device__ Row(const S* row, int vocab) : p(row), V(vocab)
+    __device__ Row(const S* row, int vocab) : p(row), V(vocab), marks(nullptr)
     {
         const int off = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(S));
         head = off ? VEC - off : 0;
         if (head > V) head = V;
         nb = (V - head) / VEC;
         const int tail0 = head + nb * VEC, t = threadIdx.x;
-        je = t < head ? t : (t >= VEC && tail0 + t - VEC < V && t < 2 * VEC ? tail0 + t - VEC : -1);
+        je = t < head ? t : (t >= VEC && t < 2 * VEC && tail0 + t - VEC < V ? tail0 + t - VEC : -1);
         xe = neg_inf();
     }
-    __device__ void load_single() { if (je >= 0) xe = E::load(p + je); }
     __device__ const u32x4* body() const { return reinterpret_cast<const u32x4*>(p + head); }
-    // f(index of the vector's first element, vector)
-    template <typename F>
-    __device__ __forceinline__ void each(F f) const
+    __device__ __forceinline__ void load()
     {
-        const u32x4* b = body();
-        for (int i = threadIdx.x; i < nb; i += NT) f(head + i * VEC, b[i]);
+        if constexpr (NV > 0) {
+            const u32x4* b = body();
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                const int i = threadIdx.x + k * NT;
+                v[k] = u32x4{E::NEG2, E::NEG2, E::NEG2, E::NEG2};
+                if (i < nb) v[k] = b[i];
+            }
+        }
+        if (je >= 0) xe = E::load(p + je);
+    }
+    // the bit map's place of class j: one bit each, the body's vectors beginning at whole bytes (nibbles for VEC = 4)
+    __device__ __forceinline__ int mark_place(int j) const { return j - head + VEC; }
+    __device__ __forceinline__ void take_out(u32x4& x, int i) const
+    {
+        const unsigned m = VEC == 8 ? marks[i + 1] : (marks[(i + 1) >> 1] >> (4 * ((i + 1) & 1))) & 15u;
+        if (m) {
+#pragma unroll
+            for (int q = 0; q < VEC; ++q)
+                if (m >> q & 1) E::clear(x, q);
+        }
+    }
+    __device__ __forceinline__ void mark(const unsigned* bits)
+    {
+        marks = reinterpret_cast<const unsigned char*>(bits);
+        if constexpr (NV > 0) {
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                const int i = threadIdx.x + k * NT;
+                if (i < nb) take_out(v[k], i);
+            }
+        }
+        if (je >= 0) {
+            const int at = mark_place(je);
+            if (bits[at >> 5] >> (at & 31) & 1) xe = neg_inf();
+        }
+    }
+    // f(index of the vector's first element, vector); ALL: also the places past the body's end, which hold -inf
+    template <bool ALL, typename F>
+    __device__ __forceinline__ void each(F f)
+    {
+        if constexpr (NV > 0) {
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                // new to the compiler in every sweep, and one vector after the other: it would otherwise keep what it
+                // unpacked for the last sweep, or unpack all vectors at once -- twice the registers, half the waves
+                asm volatile("" : "+v"(v[k]));
+                const int i = threadIdx.x + k * NT;
+                if (ALL || i < nb) f(head + i * VEC, v[k]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        } else {
+            const u32x4* b = body();
+            for (int i = threadIdx.x; i < nb; i += NT) {
+                u32x4 x = b[i];
+                if (MARKED) take_out(x, i);
+                f(head + i * VEC, x);
+            }
+        }
     }
 };
 
@@ -140,8 +208,8 @@ struct OutRow {
     __device__ __forceinline__ void one(int j, float f) const { p[j] = E::cvt(f); }
 };
 
-template <typename E, int NT>
-__device__ void fill_row(const Row<E, NT>& row, const OutRow<E>& out, float value)
+template <int NT, typename R, typename E>
+__device__ __forceinline__ void fill_row(const R& row, const OutRow<E>& out, float value)
 {
     float f[E::VEC];
 #pragma unroll
@@ -211,6 +279,53 @@ __device__ __forceinline__ int block_count(int v, int* sh)
     return v;
 }
 
+// ---- exponential and logarithm in 64 bits, for one number per row --------------------------------------------------
+// Short forms, to 1e-14 relative: the row waits in registers while they run, and the library's need as many again.
+// e^x = 2^n e^r with r = x - n ln 2, |r| <= 0.35, by its Taylor series; log x = e ln 2 + 2 atanh((m - 1) / (m + 1)) for x = 2^e m
+// with m in [sqrt(1/2), sqrt(2)], by the series of atanh, |argument| <= 0.172.
+__device__ __forceinline__ double exp_row(double x)
+{
+    const double in = fmin(fmax(x, -800.0), 800.0), n = rint(in * LOG2E);
+    const double r = fma(-n, 1.9082149292705877e-10, fma(-n, 0.6931471803691238, in));
+    double p = 1.0 / 479001600.0;
+    p = fma(p, r, 1.0 / 39916800.0);
+    p = fma(p, r, 1.0 / 3628800.0);
+    p = fma(p, r, 1.0 / 362880.0);
+    p = fma(p, r, 1.0 / 40320.0);
+    p = fma(p, r, 1.0 / 5040.0);
+    p = fma(p, r, 1.0 / 720.0);
+    p = fma(p, r, 1.0 / 120.0);
+    p = fma(p, r, 1.0 / 24.0);
+    p = fma(p, r, 1.0 / 6.0);
+    p = fma(p, r, 0.5);
+    p = fma(p, r, 1.0);
+    p = fma(p, r, 1.0);
+    return x != x ? x : ldexp(p, (int)n);
+}
+__device__ __forceinline__ double log_row(double x)
+{
+    int e;
+    double m = frexp(x, &e);
+    if (m < 0.70710678118654752) {
+        m *= 2.0;
+        e -= 1;
+    }
+    const double z = (m - 1.0) / (m + 1.0), q = z * z;
+    double p = 1.0 / 19.0;
+    p = fma(p, q, 1.0 / 17.0);
+    p = fma(p, q, 1.0 / 15.0);
+    p = fma(p, q, 1.0 / 13.0);
+    p = fma(p, q, 1.0 / 11.0);
+    p = fma(p, q, 1.0 / 9.0);
+    p = fma(p, q, 1.0 / 7.0);
+    p = fma(p, q, 1.0 / 5.0);
+    p = fma(p, q, 1.0 / 3.0);
+    p = fma(p, q, 1.0);
+    const double l = fma((double)e, 0.69314718055994531, 2.0 * z * p);
+    return x == 0.0 ? -__builtin_inf() : x == __builtin_inf() ? x : l;
+}
+__device__ __forceinline__ double from_lane(double v, int lane) { return __shfl(v, lane); }
+
 __device__ __forceinline__ float finite_or_zero(float m) { return m == neg_inf() ? 0.f : m; }
 // x - m, from below at the lowest finite number: its product with exp(-inf) = 0 is then 0 and not NaN
 __device__ __forceinline__ float clamped(float d) { return fmaxf(d, -3.402823466e38f); }
@@ -230,12 +345,28 @@ struct Rows {
 struct Weight {
     const float* gloss;
     const float* gscale;
-    const double* norm;
-    __device__ __forceinline__ double of(int64_t r) const
+    double* norm;
+    int64_t count;  // 0, or: *norm is still to be found, by counting this many rows (block 0 stores it)
+    __device__ __forceinline__ double of(int64_t r, double n) const
     {
-        return (gloss ? (double)gloss[r] : 1.0) * (gscale ? (double)*gscale : 1.0) * (norm ? *norm : 1.0);
+        return (gloss ? (double)gloss[r] : 1.0) * (gscale ? (double)*gscale : 1.0) * n;
     }
 };
+
+// The factor of the mean, in every thread.  Up to COUNT_IN_ROWS rows every block counts them itself: at most 8 KB from
+// L2 per block, against a launch and a block's latency in front of the rows (4.5 us).
+constexpr int COUNT_IN_ROWS = 1024;
+template <int NT>
+__device__ __forceinline__ double mean_norm(const Rows& rows, const Weight& w, int* sh)
+{
+    if (w.count == 0) return w.norm ? *w.norm : 1.0;
+    int n = 0;
+    for (int r = threadIdx.x; r < (int)w.count; r += NT) n += rows.kept(r) ? 1 : 0;
+    n = block_count<NT>(n, sh);
+    const double norm = n > 0 ? 1.0 / (double)n : 0.0;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *w.norm = norm;
+    return norm;
+}
 
 // 1 / (rows that count), 0 if none does.
 __global__ __launch_bounds__(1024) void count_kernel(Rows rows, int64_t R, double* __restrict__ norm)
@@ -264,31 +395,101 @@ __global__ __launch_bounds__(1024) void total_kernel(const float* __restrict__ r
     }
 }
 
-// ---- maximum, sum of exponentials and their first moment ---------------------------------------------------------
-// m = max x, s = sum exp(c (x - m)) with c in powers of two, t = sum exp(c (x - m)) (x - m): all of the row, in every thread.
-template <typename E, int NT>
-__device__ __forceinline__ void row_stats(const Row<E, NT>& row, float c, float& m, float& s, float& t, float* sh)
+// ---- maximum, sum of exponentials and a second sum -----------------------------------------------------------------
+// m = max x, s = sum exp2(c (x - m)), and by KIND a second sum: MOMENT: t = sum exp2(c (x - m)) (x - m), TWO: t = sum
+// exp2(c1 (x - m)), NONE.  All of the row, in every thread.  Each thread finds them for its own elements -- the maximum
+// first where they are in registers, all in one sweep with a running maximum where they are not -- and one reduction over
+// the block joins them; differences are taken before the scaling so that the type's lowest value in every place is a row
+// like any other.
+enum Second { NONE, MOMENT, TWO };
+template <Second KIND>
+struct Stats {
+    float m = -__builtin_inff(), s = 0.f, t = 0.f;
+
+    // to the maximum M >= m
+    __device__ __forceinline__ void raise(float M, float c, float c1)
+    {
+        if (m == neg_inf()) {
+            s = t = 0.f;
+        } else {
+            const float d = m - M, f = exp2_raw(d * c);
+            if (KIND == MOMENT) t = f == 0.f ? 0.f : f * (t + d * s);  // (d s may be infinite where f is 0)
+            if (KIND == TWO) t *= exp2_raw(d * c1);
+            s *= f;
+        }
+        m = M;
+    }
+    // me: m, or 0 where m is -inf
+    __device__ __forceinline__ void add(float x, float me, float c, float c1)
+    {
+        const float d = x - me, e = exp2_raw(d * c);
+        s += e;
+        if (KIND == MOMENT) t += e * clamped(d);
+        if (KIND == TWO) t += exp2_raw(d * c1);
+    }
+};
+
+template <Second KIND, typename E, int NT, int NV, bool MARKED>
+__device__ __forceinline__ Stats<KIND> row_stats(Row<E, NT, NV, MARKED>& row, float c, float c1, float* sh)
 {
-    float mx = row.xe;
-    row.each([&](int, const u32x4& v) {
+    Stats<KIND> a;
+    a.m = row.xe;
+    if constexpr (NV > 0) {
+        row.template each<true>([&](int, const u32x4& v) {
 #pragma unroll
-        for (int q = 0; q < E::VEC; ++q) mx = fmaxf(mx, E::get(v, q));
-    });
-    m = finite_or_zero(block_max<NT>(mx, sh));
-    const float me = m;
-    float ss = 0.f, tt = 0.f;
-    auto add = [&](float x) {
-        const float d = x - me, e = exp2f(d * c);
-        ss += e;
-        tt += e * clamped(d);
-    };
-    add(row.xe);
-    row.each([&](int, const u32x4& v) {
+            for (int q = 0; q < E::VEC; ++q) a.m = fmaxf(a.m, E::get(v, q));
+        });
+        const float me = finite_or_zero(a.m);
+        a.add(row.xe, me, c, c1);
+        row.template each<true>([&](int, const u32x4& v) {
 #pragma unroll
-        for (int q = 0; q < E::VEC; ++q) add(E::get(v, q));
-    });
-    s = block_sum<NT>(ss, sh);
-    t = block_sum<NT>(tt, sh);
+            for (int q = 0; q < E::VEC; ++q) a.add(E::get(v, q), me, c, c1);
+        });
+    } else {
+        a.add(row.xe, finite_or_zero(a.m), c, c1);
+        row.template each<true>([&](int, const u32x4& v) {
+            float vm = E::get(v, 0);
+#pragma unroll
+            for (int q = 1; q < E::VEC; ++q) vm = fmaxf(vm, E::get(v, q));
+            if (vm > a.m) a.raise(vm, c, c1);
+            const float me = finite_or_zero(a.m);
+#pragma unroll
+            for (int q = 0; q < E::VEC; ++q) a.add(E::get(v, q), me, c, c1);
+        });
+    }
+    // (the sums are needed on one side of raise()'s branch only: without this they are moved there, sweep and all)
+    asm volatile("" : "+v"(a.s), "+v"(a.t));
+    a.raise(wave_max(a.m), c, c1);
+    a.s = wave_sum(a.s);
+    if (KIND != NONE) a.t = wave_sum(a.t);
+    if (NT > 64) {
+        constexpr int NW = NT / 64;
+        const int w = threadIdx.x >> 6;
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) {
+            sh[w] = a.m;
+            sh[NW + w] = a.s;
+            if (KIND != NONE) sh[2 * NW + w] = a.t;
+        }
+        __syncthreads();
+        float M = sh[0];
+#pragma unroll
+        for (int i = 1; i < NW; ++i) M = fmaxf(M, sh[i]);
+        Stats<KIND> all;
+        all.m = M;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) {
+            Stats<KIND> b;
+            b.m = sh[i];
+            b.s = sh[NW + i];
+            b.t = KIND != NONE ? sh[2 * NW + i] : 0.f;
+            b.raise(M, c, c1);
+            all.s += b.s;
+            all.t += b.t;
+        }
+        a = all;
+    }
+    return a;
 }
 
 // ---- log-probability and entropy ---------------------------------------------------------------------------------
@@ -301,10 +502,10 @@ struct LogprobOut {
     double* logp64;
 };
 
-template <typename E, int NT>
-__global__ __launch_bounds__(NT) void logprob_kernel(Rows rows, double inv_tau, LogprobOut out)
+template <typename E, int NT, int NV>
+__global__ __launch_bounds__(NT, min_waves(NV)) void logprob_kernel(Rows rows, double inv_tau, LogprobOut out)
 {
-    __shared__ float sh[16];
+    __shared__ float sh[48];
     const int64_t r = blockIdx.x;
     if (!rows.kept(r)) {
         if (threadIdx.x == 0) {
@@ -315,13 +516,13 @@ __global__ __launch_bounds__(NT) void logprob_kernel(Rows rows, double inv_tau, 
         return;
     }
     const typename E::Store* x = reinterpret_cast<const typename E::Store*>(rows.x) + r * rows.ld;
-    Row<E, NT> row(x, rows.vocab);
-    row.load_single();
-    float m, s, t;
-    row_stats(row, (float)(LOG2E * inv_tau), m, s, t, sh);
+    Row<E, NT, NV> row(x, rows.vocab);
+    row.load();
+    const Stats<MOMENT> a = row_stats<MOMENT>(row, (float)(LOG2E * inv_tau), 0.f, sh);
     if (threadIdx.x == 0) {
+        const float m = finite_or_zero(a.m), s = a.s, t = a.t;
         const int64_t y = rows.targets[r];
-        const double log_s = log((double)s), u = -(double)t / (double)s * inv_tau;
+        const double log_s = log_row((double)s), u = -(double)t / (double)s * inv_tau;
         const double lp = (y >= 0 && y < rows.vocab) ? ((double)E::load(x + y) - (double)m) * inv_tau - log_s : __builtin_nan("");
         if (out.logp) out.logp[r] = (float)lp;
         if (out.entropy) out.entropy[r] = (float)(log_s + u);
@@ -351,13 +552,13 @@ __global__ __launch_bounds__(NT) void logprob_bwd_kernel(Rows rows, RowGrad g)
 {
     const int64_t r = blockIdx.x;
     const typename E::Store* x = reinterpret_cast<const typename E::Store*>(rows.x) + r * rows.ld;
-    Row<E, NT> row(x, rows.vocab);
+    Row<E, NT, 0> row(x, rows.vocab);
     const OutRow<E> out(g.dx, g.ldg, r, x);
     if (!rows.kept(r)) {
-        fill_row(row, out, 0.f);
+        fill_row<NT>(row, out, 0.f);
         return;
     }
-    row.load_single();
+    row.load();
     const int64_t y64 = rows.targets[r];
     const bool bad = y64 < 0 || y64 >= rows.vocab;
     const int y = bad ? -1 : (int)y64;
@@ -373,10 +574,10 @@ __global__ __launch_bounds__(NT) void logprob_bwd_kernel(Rows rows, RowGrad g)
     const float gy = gl * it, k0 = -(gl + gh * st.z) * it * st.y, k1 = -gh * it * it * st.y;
     auto value = [&](int j, float xv) {
         const float d = xv - m;
-        float v = exp2f(d * c) * (k0 + k1 * clamped(d));
+        float v = exp2_raw(d * c) * (k0 + k1 * clamped(d));
         return j == y ? v + gy : v;
     };
-    row.each([&](int j, const u32x4& v) {
+    row.template each<false>([&](int j, const u32x4& v) {
         float f[E::VEC];
 #pragma unroll
         for (int q = 0; q < E::VEC; ++q) f[q] = value(j + q, E::get(v, q));
@@ -403,50 +604,52 @@ struct Policy {
     int64_t ldg;
 };
 
-template <typename E, int NT>
-__global__ __launch_bounds__(NT) void policy_kernel(Rows rows, Policy a)
+template <typename E, int NT, int NV>
+__global__ __launch_bounds__(NT, min_waves(NV)) void policy_kernel(Rows rows, Policy a)
 {
-    __shared__ float sh[16];
+    __shared__ float sh[48];
     __shared__ float coef[3];
     if (a.skip_unit && *a.w.gscale == 1.f) return;
     const int64_t r = blockIdx.x;
     const typename E::Store* x = reinterpret_cast<const typename E::Store*>(rows.x) + r * rows.ld;
-    Row<E, NT> row(x, rows.vocab);
+    Row<E, NT, NV> row(x, rows.vocab);
     const OutRow<E> out(a.dx, a.ldg, r, x);
+    const double norm = mean_norm<NT>(rows, a.w, reinterpret_cast<int*>(sh));
     if (!rows.kept(r)) {
         if (threadIdx.x == 0) {
             if (a.row_loss) a.row_loss[r] = 0.f;
             if (a.logp) a.logp[r] = 0.f;
             if (a.entropy) a.entropy[r] = 0.f;
         }
-        if (a.dx) fill_row(row, out, 0.f);
+        if (a.dx) fill_row<NT>(row, out, 0.f);
         return;
     }
-    row.load_single();
-    float m, s, t;
+    row.load();
     const float c = (float)(LOG2E * a.inv_tau);
-    row_stats(row, c, m, s, t, sh);
+    const Stats<MOMENT> all = row_stats<MOMENT>(row, c, 0.f, sh);
+    const float m = finite_or_zero(all.m), s = all.s, t = all.t;
     const int64_t y64 = rows.targets[r];
     const int y = (y64 >= 0 && y64 < rows.vocab) ? (int)y64 : -1;
-    if (threadIdx.x == 0) {
-        const double it = a.inv_tau, log_s = log((double)s), u = -(double)t / (double)s * it, H = log_s + u;
+    if (threadIdx.x < 64) {
+        const double it = a.inv_tau, log_s = log_row((double)s), u = -(double)t / (double)s * it, H = log_s + u;
         const double lp = y >= 0 ? ((double)E::load(x + y) - (double)m) * it - log_s : __builtin_nan("");
-        const double A = (double)a.adv[r % a.adv_rows];
-        const double rho = exp(lp - (double)a.old_logp[r]);
+        const double A = (double)a.adv[r % a.adv_rows], gap = a.ref_logp ? (double)a.ref_logp[r] - lp : 0.0;
+        // two exponentials, side by side in two lanes
+        const double both = exp_row(threadIdx.x == 0 ? lp - (double)a.old_logp[r] : gap);
+        const double rho = from_lane(both, 0), away = from_lane(both, 1);
         const double free = rho * A, held = (rho < a.lo ? a.lo : rho > a.hi ? a.hi : rho) * A;
         double loss = free <= held ? -free : -held, g = free <= held ? -free : 0.0;
         if (free != free) loss = g = free;  // a NaN stays one
         if (a.ref_logp) {
-            const double gap = (double)a.ref_logp[r] - lp, away = exp(gap);
             loss += a.kl * (away - gap - 1.0);
             g += a.kl * (1.0 - away);
         }
         if (a.ent != 0.0) loss -= a.ent * H;
-        if (a.row_loss) a.row_loss[r] = (float)loss;
-        if (a.logp) a.logp[r] = (float)lp;
-        if (a.entropy) a.entropy[r] = (float)H;
-        if (a.dx) {
-            const double w = a.w.of(r) * it;
+        if (threadIdx.x == 0) {
+            if (a.row_loss) a.row_loss[r] = (float)loss;
+            if (a.logp) a.logp[r] = (float)lp;
+            if (a.entropy) a.entropy[r] = (float)H;
+            const double w = a.w.of(r, norm) * it;
             coef[0] = (float)(w * (-g + a.ent * u) / (double)s);
             coef[1] = (float)(w * a.ent * it / (double)s);
             coef[2] = (float)(w * g);
@@ -457,10 +660,10 @@ __global__ __launch_bounds__(NT) void policy_kernel(Rows rows, Policy a)
     const float k0 = coef[0], k1 = coef[1], gy = coef[2];
     auto value = [&](int j, float xv) {
         const float d = xv - m;
-        float v = exp2f(d * c) * (k0 + k1 * clamped(d));
+        float v = exp2_raw(d * c) * (k0 + k1 * clamped(d));
         return j == y ? v + gy : v;
     };
-    row.each([&](int j, const u32x4& v) {
+    row.template each<false>([&](int j, const u32x4& v) {
         float f[E::VEC];
 #pragma unroll
         for (int q = 0; q < E::VEC; ++q) f[q] = value(j + q, E::get(v, q));
@@ -503,11 +706,11 @@ __device__ __forceinline__ float load_as(const void* p, int type, int64_t i)
     return (float)reinterpret_cast<const __bf16*>(p)[i];
 }
 
-template <typename E, int NT, bool TWO>
-__global__ __launch_bounds__(NT) void distill_kernel(Rows rows, Distill a)
+template <typename E, int NT, int NV, bool BOTH>
+__global__ __launch_bounds__(NT, min_waves(NV)) void distill_kernel(Rows rows, Distill a)
 {
-    extern __shared__ unsigned bits[];  // (vocab + 31) / 32
-    __shared__ float sh[16];
+    extern __shared__ unsigned bits[];  // a bit per class, see Row::mark_place: (vocab + 2 VEC + 31) / 32
+    __shared__ float sh[48];
     __shared__ int sidx[DISTILL_MAX_K];    // class, -1 where the entry takes no part
     __shared__ float st[DISTILL_MAX_K], sx[DISTILL_MAX_K], sq[DISTILL_MAX_K];
     __shared__ unsigned char own[DISTILL_MAX_K];
@@ -518,33 +721,47 @@ __global__ __launch_bounds__(NT) void distill_kernel(Rows rows, Distill a)
     if (a.skip_unit && *a.w.gscale == 1.f) return;
     const int64_t r = blockIdx.x;
     const typename E::Store* x = reinterpret_cast<const typename E::Store*>(rows.x) + r * rows.ld;
-    Row<E, NT> row(x, rows.vocab);
+    Row<E, NT, NV, true> row(x, rows.vocab);
     const OutRow<E> out(a.dx, a.ldg, r, x);
+    const double norm = mean_norm<NT>(rows, a.w, reinterpret_cast<int*>(sh));
     if (!rows.kept(r)) {
         if (threadIdx.x == 0 && a.row_loss) a.row_loss[r] = 0.f;
-        if (a.dx) fill_row(row, out, 0.f);
+        if (a.dx) fill_row<NT>(row, out, 0.f);
         return;
     }
     const int tid = threadIdx.x;
     const int64_t y64 = rows.targets[r];
     const int y = (y64 >= 0 && y64 < rows.vocab) ? (int)y64 : -1;
-    for (int i = tid; i < (rows.vocab + 31) / 32; i += NT) bits[i] = 0;
+    // the list first: its loads are the ones that others wait for
+    constexpr int KP = (DISTILL_MAX_K + NT - 1) / NT;
+    int jk[KP];
+#pragma unroll
+    for (int i = 0; i < KP; ++i) {
+        const int k = tid + i * NT;
+        jk[i] = k < a.k ? a.indices[r * a.k + k] : -1;
+    }
+    row.load();
+    for (int i = tid; i < (rows.vocab + 2 * E::VEC + 31) / 32; i += NT) bits[i] = 0;
     if (tid == 0) {
         bad = y < 0;
         twice = 0;
     }
     __syncthreads();
-    for (int k = tid; k < a.k; k += NT) {
-        const int j = a.indices[r * a.k + k];
+#pragma unroll
+    for (int i = 0; i < KP; ++i) {
+        const int k = tid + i * NT, j = jk[i];
+        if (k >= a.k) continue;
         const bool in = j >= 0 && j < rows.vocab;
         if (j >= rows.vocab) bad = 1;  // (every writer writes the same value)
         sidx[k] = in ? j : -1;
         st[k] = in ? load_as(a.values, a.value_type, r * a.k + k) : neg_inf();
         sx[k] = in ? E::load(x + j) : neg_inf();
         own[k] = in;
-        if (in && (atomicOr(&bits[j >> 5], 1u << (j & 31)) >> (j & 31) & 1) != 0) twice = 1;
+        if (in) {
+            const int at = row.mark_place(j);
+            if (atomicOr(&bits[at >> 5], 1u << (at & 31)) >> (at & 31) & 1) twice = 1;
+        }
     }
-    row.load_single();
     __syncthreads();
     if (twice) {  // of a class listed more than once the first entry stands for all: in a fixed order, so sums repeat
         for (int k = tid; k < a.k; k += NT)
@@ -552,31 +769,12 @@ __global__ __launch_bounds__(NT) void distill_kernel(Rows rows, Distill a)
                 if (sidx[i] == sidx[k]) own[k] = 0;
         __syncthreads();
     }
-    auto listed = [&](int j) { return (bits[j >> 5] >> (j & 31) & 1) != 0; };
-    const float xe = row.je >= 0 && !listed(row.je) ? row.xe : neg_inf();
+    row.mark(bits);
 
     // the classes outside the list: maximum, sums at both temperatures
-    float mx = xe;
-    row.each([&](int j, const u32x4& v) {
-#pragma unroll
-        for (int q = 0; q < E::VEC; ++q) mx = fmaxf(mx, listed(j + q) ? neg_inf() : E::get(v, q));
-    });
-    const float m_rest = block_max<NT>(mx, sh);
-    const float mt = finite_or_zero(m_rest);
     const float c = (float)(LOG2E * a.inv_tau), c1 = (float)LOG2E;
-    float s_tau = 0.f, s_one = 0.f;
-    auto add = [&](float xv) {
-        const float d = xv - mt;
-        s_tau += exp2f(d * c);
-        if (TWO) s_one += exp2f(d * c1);
-    };
-    add(xe);
-    row.each([&](int j, const u32x4& v) {
-#pragma unroll
-        for (int q = 0; q < E::VEC; ++q) add(listed(j + q) ? neg_inf() : E::get(v, q));
-    });
-    s_tau = block_sum<NT>(s_tau, sh);
-    s_one = TWO ? block_sum<NT>(s_one, sh) : s_tau;
+    const auto rest = row_stats<BOTH ? TWO : NONE>(row, c, c1, sh);
+    const float m_rest = rest.m, mt = finite_or_zero(rest.m), s_tau = rest.s, s_one = BOTH ? rest.t : rest.s;
 
     // one wave: the teacher's distribution, the student's sums over everything, the loss
     if (tid < 64) {
@@ -594,46 +792,49 @@ __global__ __launch_bounds__(NT) void distill_kernel(Rows rows, Distill a)
         double z = 0.0, s = 0.0, s1 = 0.0, cross = 0.0;
         for (int k = tid; k < a.k; k += 64) {
             const double u = (double)st[k] * it;
-            const float q = exp2f((float)((u - M) * LOG2E));
+            const float q = exp2_raw((float)((u - M) * LOG2E));
             sq[k] = q;
             z += (double)q;
             if (q != 0.f) cross += (double)q * ((u - M) - ((double)sx[k] - (double)m) * it);
             if (own[k]) {
-                s += (double)exp2f((sx[k] - m) * c);
-                if (TWO) s1 += (double)exp2f((sx[k] - m) * c1);
+                s += (double)exp2_raw((sx[k] - m) * c);
+                if (BOTH) s1 += (double)exp2_raw((sx[k] - m) * c1);
             }
         }
         z = wave_sum(z);
         s = wave_sum(s);
-        s1 = TWO ? wave_sum(s1) : 0.0;
+        s1 = BOTH ? wave_sum(s1) : 0.0;
         cross = wave_sum(cross);
-        const double qt0 = tail > -1e300 || tail != tail ? exp(tail - M) : 0.0;
-        z += qt0;
-        // exp of (the others' maximum) - (the row's): in 64 bits, for it scales every class outside the list
+        // exponentials and logarithms side by side in the wave's lanes; those that scale every class outside the list,
+        // of (the others' maximum) - (the row's), in 64 bits like the rest
         const double gap = (double)m_rest - (double)m;
-        const double lift = exp(gap * it), lift1 = TWO ? exp(gap) : lift;
+        const double e3 = exp_row(tid == 0 ? tail - M : tid == 1 ? gap * it : gap);
+        const double qt0 = from_lane(e3, 0), lift = from_lane(e3, 1), lift1 = BOTH ? from_lane(e3, 2) : lift;
+        z += qt0;
         s += (double)s_tau * lift;
-        s1 = TWO ? s1 + (double)s_one * lift1 : s;
+        s1 = BOTH ? s1 + (double)s_one * lift1 : s;
+        const double l4 = log_row(tid == 0 ? z : tid == 1 ? s : tid == 2 ? (double)s_tau : s1);
+        const double log_z = from_lane(l4, 0), log_s = from_lane(l4, 1), log_rest = from_lane(l4, 2), log_s1 = from_lane(l4, 3);
         const bool none = z == 0.0;  // the teacher says nothing about this row
         const double qt = none ? 0.0 : qt0 / z;
         double kd = 0.0;
         const double wkd = 1.0 - a.ce;
         if (!none && wkd != 0.0) {
             // everything relative to the two maxima M and m, which may be as large as the type's lowest value
-            kd = cross / z - (log(z) - log(s));
-            if (qt != 0.0) kd += qt * ((tail - M) - (log((double)s_tau) + gap * it));
+            kd = cross / z - (log_z - log_s);
+            if (qt != 0.0) kd += qt * ((tail - M) - (log_rest + gap * it));
             kd *= wkd * a.tau * a.tau;
         }
         double ce = 0.0;
-        if (a.ce != 0.0 && y >= 0) ce = a.ce * (log(s1) - ((double)E::load(x + y) - (double)m));
+        if (a.ce != 0.0 && y >= 0) ce = a.ce * (log_s1 - ((double)E::load(x + y) - (double)m));
         if (tid == 0) {
             double loss = kd + ce;
             if (bad) loss = __builtin_nan("");
             if (a.row_loss) a.row_loss[r] = (float)loss;
-            const double w = bad ? __builtin_nan("") : a.w.of(r);
+            const double w = bad ? __builtin_nan("") : a.w.of(r, norm);
             const double wk = none || wkd == 0.0 ? 0.0 : w * wkd * a.tau, wc = w * a.ce;
             const double ka = wk == 0.0 ? 0.0 : wk * (lift / s - (qt != 0.0 ? qt / (double)s_tau : 0.0)), kb = wc * lift1 / s1;
-            coef[0] = (float)(TWO ? ka : ka + kb);
+            coef[0] = (float)(BOTH ? ka : ka + kb);
             coef[1] = (float)kb;
             coef[2] = (float)wc;
             glob[0] = wk / s;                   // of exp((x_k - m) / tau)
@@ -647,11 +848,11 @@ __global__ __launch_bounds__(NT) void distill_kernel(Rows rows, Distill a)
     const float ka = coef[0], kb = coef[1], gy = coef[2];
     auto value = [&](int j, float xv) {
         const float d = xv - mt;
-        float v = exp2f(d * c) * ka;
-        if (TWO) v += exp2f(d * c1) * kb;
+        float v = exp2_raw(d * c) * ka;
+        if (BOTH) v += exp2_raw(d * c1) * kb;
         return j == y ? v - gy : v;
     };
-    row.each([&](int j, const u32x4& v) {
+    row.template each<false>([&](int j, const u32x4& v) {
         float f[E::VEC];
 #pragma unroll
         for (int q = 0; q < E::VEC; ++q) f[q] = value(j + q, E::get(v, q));
@@ -666,8 +867,8 @@ __global__ __launch_bounds__(NT) void distill_kernel(Rows rows, Distill a)
             for (int i = k + 1; i < a.k; ++i)
                 if (sidx[i] == sidx[k]) q += sq[i];
         const float d = sx[k] - (float)glob[3];
-        double v = (double)exp2f(d * c) * glob[0] - (double)q * glob[1];
-        if (a.ce != 0.0) v += (double)exp2f(d * c1) * glob[2];
+        double v = (double)exp2_raw(d * c) * glob[0] - (double)q * glob[1];
+        if (a.ce != 0.0) v += (double)exp2_raw(d * c1) * glob[2];
         if (sidx[k] == y) v -= (double)gy;
         out.one(sidx[k], (float)v);
     }
@@ -676,92 +877,207 @@ __global__ __launch_bounds__(NT) void distill_kernel(Rows rows, Distill a)
 // ---- the k largest logits of a row --------------------------------------------------------------------------------
 // Exact: larger first, equal ones by ascending index (-0 equals +0, a NaN is larger than every number).  The k-th
 // largest is found bit by bit on integers in the order of the values, ties by bits of the index.
-constexpr int TOP_MAX_K = 256;
-
 __device__ __forceinline__ unsigned order_key(float x)
 {
     const unsigned b = __float_as_uint(x + 0.f);
     return x != x ? 0xffffffffu : (b & 0x80000000u) ? ~b : b | 0x80000000u;
 }
 
-template <typename E, int NT>
-__global__ __launch_bounds__(NT) void top_kernel(const void* logits, int64_t ld, int V, int k, double inv_tau,
+// The usual way takes two sweeps.  The first finds every thread's two maxima (over the vectors' halves): the k-th largest
+// of those, 2 NT numbers, is a bound that at least k elements reach and, for k well below 2 NT, few more do.  The second
+// puts what reaches the bound on a list and sums the exponentials of everything below, relative to the bound.  The list's
+// elements then find their rank by comparing with each other.  Where the list would overflow (many equal values), or a
+// NaN is about, the k-th largest is found bit by bit with a sweep for each; where what lies below the bound vanishes
+// beside it, the tail is summed in two more sweeps relative to its own maximum.
+constexpr int TOP_LIST = 1024;
+
+__device__ __forceinline__ float key_value(unsigned key)  // the float of a key that is no NaN's
+{
+    return __uint_as_float((key & 0x80000000u) ? key ^ 0x80000000u : ~key);
+}
+
+template <typename E, int NT, int NV>
+__global__ __launch_bounds__(NT, min_waves(NV)) void top_kernel(const void* logits, int64_t ld, int V, int k, double inv_tau,
                                                  void* __restrict__ values, int32_t* __restrict__ indices,
                                                  float* __restrict__ tail)
 {
     __shared__ float shf[16];
     __shared__ int sh[16];
     __shared__ int fill;
-    __shared__ unsigned ckey[TOP_MAX_K];
-    __shared__ int cidx[TOP_MAX_K];
+    __shared__ unsigned bound_key, kth_key;
+    __shared__ int kth_idx;
+    __shared__ unsigned ckey[TOP_LIST];
+    __shared__ int cidx[TOP_LIST];
+    __shared__ float rest[TOP_LIST];     // listed but not among the k, in order
+    __shared__ unsigned maxima[2 * NT];
     const int64_t r = blockIdx.x;
     const int tid = threadIdx.x;
     const typename E::Store* x = reinterpret_cast<const typename E::Store*>(logits) + r * ld;
-    Row<E, NT> row(x, V);
-    row.load_single();
-    auto count = [&](auto pred) {
-        int n = row.je >= 0 && pred(row.je, row.xe) ? 1 : 0;
-        row.each([&](int j, const u32x4& v) {
+    Row<E, NT, NV> row(x, V);
+    row.load();
+    const float c = (float)(LOG2E * inv_tau);
+
+    float lo = row.xe, hi = neg_inf();
+    row.template each<true>([&](int, const u32x4& v) {
 #pragma unroll
-            for (int q = 0; q < E::VEC; ++q) n += pred(j + q, E::get(v, q)) ? 1 : 0;
-        });
-        return block_count<NT>(n, sh);
-    };
-    unsigned kth = 0;  // the largest key that at least k elements reach
-    for (int bit = 31; bit >= 0; --bit) {
-        const unsigned cand = kth | (1u << bit);
-        if (count([&](int, float v) { return order_key(v) >= cand; }) >= k) kth = cand;
-    }
-    const int need = k - count([&](int, float v) { return order_key(v) > kth; });
-    int last = 0;  // the need-th element of that key, by index
-    for (int bit = 30; bit >= 0; --bit) {
-        const int cand = last + (1 << bit);
-        if (cand < V && count([&](int j, float v) { return j < cand && order_key(v) == kth; }) < need) last = cand;
-    }
-    auto chosen = [&](int j, float v) {
-        const unsigned key = order_key(v);
-        return key > kth || (key == kth && j <= last);
-    };
+        for (int q = 0; q < E::VEC / 2; ++q) {
+            lo = fmaxf(lo, E::get(v, q));
+            hi = fmaxf(hi, E::get(v, q + E::VEC / 2));
+        }
+    });
+    maxima[tid] = order_key(lo);
+    maxima[NT + tid] = order_key(hi);
     if (tid == 0) fill = 0;
     __syncthreads();
-    auto take = [&](int j, float v) {
-        if (chosen(j, v)) {
-            const int at = atomicAdd(&fill, 1);
-            ckey[at] = order_key(v);
+    if (tid < 64) {
+        // the k-th largest maximum to 16 bits, rounded down
+        unsigned mk[2 * NT / 64];
+#pragma unroll
+        for (int i = 0; i < 2 * NT / 64; ++i) mk[i] = maxima[tid + 64 * i];
+        unsigned kth = 0;
+#pragma unroll 1
+        for (unsigned bit = 0x80000000u; bit >= 0x10000u; bit >>= 1) {
+            const unsigned cand = kth | bit;
+            int n = 0;
+#pragma unroll
+            for (int i = 0; i < 2 * NT / 64; ++i) n += __popcll(__ballot(mk[i] >= cand));
+            if (n >= k) kth = cand;
+        }
+        if (tid == 0) bound_key = kth;
+    }
+    __syncthreads();
+    const float bound = bound_key > order_key(neg_inf()) ? key_value(bound_key) : neg_inf();
+    auto put = [&](int j, float f) {
+        const int at = atomicAdd(&fill, 1);
+        if (at < TOP_LIST) {
+            ckey[at] = order_key(f);
             cidx[at] = j;
         }
     };
-    if (row.je >= 0) take(row.je, row.xe);
-    float mx = row.je >= 0 && !chosen(row.je, row.xe) ? row.xe : neg_inf();
-    row.each([&](int j, const u32x4& v) {
-#pragma unroll
-        for (int q = 0; q < E::VEC; ++q) {
-            const float f = E::get(v, q);
-            take(j + q, f);
-            if (!chosen(j + q, f)) mx = fmaxf(mx, f);
-        }
-    });
-    const float m_rest = block_max<NT>(mx, shf);  // (its barriers also close the list)
-    const float m = finite_or_zero(m_rest);
     float s = 0.f;
-    const float c = (float)(LOG2E * inv_tau);
-    if (row.je >= 0 && !chosen(row.je, row.xe)) s += exp2f((row.xe - m) * c);
-    row.each([&](int j, const u32x4& v) {
+    auto below = [&](float f) { s += exp2_raw((f - bound) * c); };
+    if (row.je >= 0) {
+        if (row.xe < bound) below(row.xe);
+        else put(row.je, row.xe);
+    }
+    row.template each<false>([&](int j, const u32x4& v) {
+        float vm = E::get(v, 0);
 #pragma unroll
-        for (int q = 0; q < E::VEC; ++q) {
-            const float f = E::get(v, q);
-            if (!chosen(j + q, f)) s += exp2f((f - m) * c);
+        for (int q = 1; q < E::VEC; ++q) vm = fmaxf(vm, E::get(v, q));
+        if (vm < bound) {
+#pragma unroll
+            for (int q = 0; q < E::VEC; ++q) below(E::get(v, q));  // (a NaN among them shows in the sum)
+        } else {
+#pragma unroll
+            for (int q = 0; q < E::VEC; ++q) {
+                const float f = E::get(v, q);
+                if (f < bound) below(f);
+                else put(j + q, f);
+            }
         }
     });
     s = block_sum<NT>(s, shf);
-    if (tid == 0) tail[r] = m_rest == __builtin_inff() && s != s ? m_rest : (float)(log((double)s) + (double)m * inv_tau);
     __syncthreads();
-    for (int i = tid; i < k; i += NT) {
-        int rank = 0;
-        for (int o = 0; o < k; ++o) rank += ckey[o] > ckey[i] || (ckey[o] == ckey[i] && cidx[o] < cidx[i]) ? 1 : 0;
-        indices[r * k + rank] = cidx[i];
-        reinterpret_cast<typename E::Store*>(values)[r * k + rank] = x[cidx[i]];
+    int n = fill;
+    const bool exact = n > TOP_LIST || s != s;
+    Row<E, NT, 0> again(x, V);  // the rare ways read the row anew: their loops need no registers of the usual one's
+    if (exact) {
+        again.load();
+        auto count = [&](auto pred) {
+            int cnt = again.je >= 0 && pred(again.je, again.xe) ? 1 : 0;
+            again.template each<false>([&](int j, const u32x4& v) {
+#pragma unroll
+                for (int q = 0; q < E::VEC; ++q) cnt += pred(j + q, E::get(v, q)) ? 1 : 0;
+            });
+            return block_count<NT>(cnt, sh);
+        };
+        unsigned kth = 0;  // the largest key that at least k elements reach
+        for (int bit = 31; bit >= 0; --bit) {
+            const unsigned cand = kth | (1u << bit);
+            if (count([&](int, float v) { return order_key(v) >= cand; }) >= k) kth = cand;
+        }
+        const int need = k - count([&](int, float v) { return order_key(v) > kth; });
+        int last = 0;  // the need-th element of that key, by index
+        for (int bit = 30; bit >= 0; --bit) {
+            const int cand = last + (1 << bit);
+            if (cand < V && count([&](int j, float v) { return j < cand && order_key(v) == kth; }) < need) last = cand;
+        }
+        __syncthreads();
+        if (tid == 0) fill = 0;
+        __syncthreads();
+        auto take = [&](int j, float f) {
+            const unsigned key = order_key(f);
+            if (key > kth || (key == kth && j <= last)) put(j, f);
+        };
+        if (again.je >= 0) take(again.je, again.xe);
+        again.template each<false>([&](int j, const u32x4& v) {
+#pragma unroll
+            for (int q = 0; q < E::VEC; ++q) take(j + q, E::get(v, q));
+        });
+        __syncthreads();
+        n = k;
     }
+    for (int i = tid; i < n; i += NT) {
+        const unsigned ki = ckey[i];
+        const int ji = cidx[i];
+        int rank = 0;
+        for (int o = 0; o < n; ++o) rank += ckey[o] > ki || (ckey[o] == ki && cidx[o] < ji) ? 1 : 0;
+        if (rank < k) {
+            indices[r * k + rank] = ji;
+            reinterpret_cast<typename E::Store*>(values)[r * k + rank] = x[ji];
+            if (rank == k - 1) {
+                kth_key = ki;
+                kth_idx = ji;
+            }
+        } else {
+            rest[rank - k] = key_value(ki);
+        }
+    }
+    __syncthreads();
+    if (!exact && (s > 1e-30f || n == V)) {
+        // what lies below the bound, and the list's own remainder relative to its first
+        if (tid < 64) {
+            const float first = n > k ? rest[0] : neg_inf();
+            float t = 0.f;
+            for (int i = tid; i < n - k; i += 64) t += first == neg_inf() ? 0.f : exp2_raw((rest[i] - first) * c);
+            t = wave_sum(t);
+            if (tid == 0) {
+                const double top = fmax((double)first, s > 0.f ? (double)bound : (double)neg_inf());
+                double sum = 0.0;
+                if (s > 0.f) sum += (double)s * exp_row(((double)bound - top) * inv_tau);
+                if (t > 0.f) sum += (double)t * exp_row(((double)first - top) * inv_tau);
+                // (an infinite first, and a NaN, which is before every number, are the sum themselves)
+                tail[r] = first == __builtin_inff() || first != first ? first : sum > 0.0 ? (float)(top * inv_tau + log_row(sum)) : neg_inf();
+            }
+        }
+        return;
+    }
+    const unsigned kth = kth_key;
+    const int last = kth_idx;
+    auto chosen = [&](int j, float f) {
+        const unsigned key = order_key(f);
+        return key > kth || (key == kth && j <= last);
+    };
+    again.load();
+    float mx = again.je >= 0 && !chosen(again.je, again.xe) ? again.xe : neg_inf();
+    again.template each<false>([&](int j, const u32x4& v) {
+#pragma unroll
+        for (int q = 0; q < E::VEC; ++q) {
+            const float f = E::get(v, q);
+            if (!chosen(j + q, f)) mx = fmaxf(mx, f);
+        }
+    });
+    const float m_rest = block_max<NT>(mx, shf), m = finite_or_zero(m_rest);
+    s = again.je >= 0 && !chosen(again.je, again.xe) ? exp2_raw((again.xe - m) * c) : 0.f;
+    again.template each<false>([&](int j, const u32x4& v) {
+#pragma unroll
+        for (int q = 0; q < E::VEC; ++q) {
+            const float f = E::get(v, q);
+            if (!chosen(j + q, f)) s += exp2_raw((f - m) * c);
+        }
+    });
+    s = block_sum<NT>(s, shf);
+    if (tid == 0) tail[r] = m_rest == __builtin_inff() && s != s ? m_rest : (float)(log_row((double)s) + (double)m * inv_tau);
 }
 
 // ---- preference loss over pairs of sequences -------------------------------------------------------------------------
@@ -826,27 +1142,31 @@ __global__ __launch_bounds__(1024) void prefer_kernel(Prefer a)
     }
 }
 
-// A block per row: as many threads as the row's vectors keep busy.
-#define GTG_BY_SIZE(DTYPE, VOCAB, CALL)                                  \
-    do {                                                                 \
-        const int64_t bytes_ = (int64_t)(VOCAB) * ((DTYPE) == GTG_DTYPE_F32 ? 4 : 2); \
-        if ((DTYPE) == GTG_DTYPE_F32) {                                  \
-            typedef F32 E;                                               \
-            if (bytes_ <= 4096) { constexpr int NT = 64; CALL; }         \
-            else if (bytes_ <= 32768) { constexpr int NT = 256; CALL; }  \
-            else { constexpr int NT = 512; CALL; }                       \
-        } else if ((DTYPE) == GTG_DTYPE_F16) {                           \
-            typedef F16 E;                                               \
-            if (bytes_ <= 4096) { constexpr int NT = 64; CALL; }         \
-            else if (bytes_ <= 32768) { constexpr int NT = 256; CALL; }  \
-            else { constexpr int NT = 512; CALL; }                       \
-        } else {                                                         \
-            typedef BF16 E;                                              \
-            if (bytes_ <= 4096) { constexpr int NT = 64; CALL; }         \
-            else if (bytes_ <= 32768) { constexpr int NT = 256; CALL; }  \
-            else { constexpr int NT = 512; CALL; }                       \
-        }                                                                \
-    } while (0)
+// A block per row, by the row's 16-byte vectors: as many threads as they keep busy, and the row in registers up to 16 vectors
+// (64 registers) a thread and 1024 threads -- 128 K elements of 16 bits, 64 K of 32.
+template <typename E_, int NT_, int NV_>
+struct Shape {
+    typedef E_ E;
+    static constexpr int NT = NT_, NV = NV_;
+};
+template <typename E, typename F>
+void by_vectors(int64_t n, F launch)
+{
+    if (n <= 64) launch(Shape<E, 64, 1>());
+    else if (n <= 256) launch(Shape<E, 64, 4>());
+    else if (n <= 1024) launch(Shape<E, 256, 4>());
+    else if (n <= 4096) launch(Shape<E, 512, 8>());
+    else if (n <= 8192) launch(Shape<E, 512, 16>());
+    else if (n <= 16384) launch(Shape<E, 1024, 16>());
+    else launch(Shape<E, 512, 0>());
+}
+template <typename F>
+void by_size(int dtype, int vocab, F launch)
+{
+    if (dtype == GTG_DTYPE_F32) by_vectors<F32>(((int64_t)vocab + 3) / 4, launch);
+    else if (dtype == GTG_DTYPE_F16) by_vectors<F16>(((int64_t)vocab + 7) / 8, launch);
+    else by_vectors<BF16>(((int64_t)vocab + 7) / 8, launch);
+}
 
 Rows as_rows(const TokenRows& t) { return Rows{t.logits, t.ld, t.vocab, t.targets, t.padidx, t.mask}; }
 
@@ -857,8 +1177,10 @@ int top_logits(const void* logits, int dtype, int64_t R, int V, int64_t ld, int 
 {
     ProfScope prof(s, "top_logits", R, V, k);
     const double it = 1.0 / temperature;
-    GTG_BY_SIZE(dtype, V, hipLaunchKernelGGL(HIP_KERNEL_NAME(top_kernel<E, NT>), dim3((unsigned)R), dim3(NT), 0, s, logits, ld, V,
-                                             k, it, values, indices, tail));
+    by_size(dtype, V, [&](auto shape) {
+        typedef decltype(shape) P;
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(top_kernel<typename P::E, P::NT, P::NV>), dim3((unsigned)R), dim3(P::NT), 0, s, logits, ld, V, k, it, values, indices, tail);
+    });
     return check_launch("top_kernel");
 }
 
@@ -868,8 +1190,10 @@ int token_logprob_fwd(const TokenRows& t, double temperature, float* logp, float
     ProfScope prof(s, "token_logprob_fwd", t.rows, t.vocab, 0);
     const LogprobOut out{logp, entropy, reinterpret_cast<float4*>(stats), logp64};
     const double it = 1.0 / temperature;
-    GTG_BY_SIZE(t.dtype, t.vocab, hipLaunchKernelGGL(HIP_KERNEL_NAME(logprob_kernel<E, NT>), dim3((unsigned)t.rows), dim3(NT), 0,
-                                                     s, as_rows(t), it, out));
+    by_size(t.dtype, t.vocab, [&](auto shape) {
+        typedef decltype(shape) P;
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(logprob_kernel<typename P::E, P::NT, P::NV>), dim3((unsigned)t.rows), dim3(P::NT), 0, s, as_rows(t), it, out);
+    });
     return check_launch("logprob_kernel");
 }
 
@@ -879,10 +1203,14 @@ int token_logprob_bwd(const TokenRows& t, double temperature, const float* stats
 {
     ProfScope prof(s, "token_logprob_bwd", t.rows, t.vocab, 0);
     const RowGrad g{reinterpret_cast<const float4*>(stats), g_logp, g_entropy, gscale, gloss, group, pairs, 1.0 / temperature, dx, ldg};
-    GTG_BY_SIZE(t.dtype, t.vocab, hipLaunchKernelGGL(HIP_KERNEL_NAME(logprob_bwd_kernel<E, NT>), dim3((unsigned)t.rows), dim3(NT),
-                                                     0, s, as_rows(t), g));
+    by_size(t.dtype, t.vocab, [&](auto shape) {
+        typedef decltype(shape) P;
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(logprob_bwd_kernel<typename P::E, P::NT>), dim3((unsigned)t.rows), dim3(P::NT), 0, s, as_rows(t), g);
+    });
     return check_launch("logprob_bwd_kernel");
 }
+
+bool counts_in_rows(int64_t R) { return R <= COUNT_IN_ROWS; }
 
 int count_rows(const TokenRows& t, double* norm, hipStream_t s)
 {
@@ -896,32 +1224,39 @@ int total_loss(const float* row_loss, int64_t R, const double* norm, float* loss
     return check_launch("total_kernel");
 }
 
-int policy_rows(const TokenRows& t, const PolicyRows& p, const float* gloss, const float* gscale, const double* norm,
+int policy_rows(const TokenRows& t, const PolicyRows& p, const float* gloss, const float* gscale, double* norm, bool count,
                 bool skip_unit, float* row_loss, float* logp, float* entropy, void* dx, int64_t ldg, hipStream_t s)
 {
     ProfScope prof(s, "policy_rows", t.rows, t.vocab, dx != nullptr);
     const Policy a{p.old_logp, p.advantages, p.adv_rows, p.ref_logp, 1.0 - p.clip_low, 1.0 + p.clip_high, p.kl_coef, p.entropy_coef,
-                   1.0 / p.temperature, Weight{gloss, gscale, norm}, skip_unit ? 1 : 0, row_loss, logp, entropy, dx, ldg};
-    GTG_BY_SIZE(t.dtype, t.vocab, hipLaunchKernelGGL(HIP_KERNEL_NAME(policy_kernel<E, NT>), dim3((unsigned)t.rows), dim3(NT), 0, s,
-                                                     as_rows(t), a));
+                   1.0 / p.temperature, Weight{gloss, gscale, norm, count ? t.rows : 0}, skip_unit ? 1 : 0, row_loss, logp, entropy, dx, ldg};
+    by_size(t.dtype, t.vocab, [&](auto shape) {
+        typedef decltype(shape) P;
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(policy_kernel<typename P::E, P::NT, P::NV>), dim3((unsigned)t.rows), dim3(P::NT), 0, s, as_rows(t), a);
+    });
     return check_launch("policy_kernel");
 }
 
 int distill_max_vocab() { return DISTILL_MAX_VOCAB; }
 
-int distill_rows(const TokenRows& t, const DistillRows& d, const float* gloss, const float* gscale, const double* norm,
+int distill_rows(const TokenRows& t, const DistillRows& d, const float* gloss, const float* gscale, double* norm, bool count,
                  bool skip_unit, float* row_loss, void* dx, int64_t ldg, hipStream_t s)
 {
     ProfScope prof(s, "distill_rows", t.rows, t.vocab, dx != nullptr);
     const Distill a{d.values, d.value_dtype, d.indices, d.k, d.tail, 1.0 / d.temperature, d.temperature, d.ce_weight,
-                    Weight{gloss, gscale, norm}, skip_unit ? 1 : 0, row_loss, dx, ldg};
-    const size_t lds = (size_t)((t.vocab + 31) / 32) * 4;
-    if (d.ce_weight != 0.0 && d.temperature != 1.0)
-        GTG_BY_SIZE(t.dtype, t.vocab, hipLaunchKernelGGL(HIP_KERNEL_NAME(distill_kernel<E, NT, true>), dim3((unsigned)t.rows), dim3(NT),
-                                                         lds, s, as_rows(t), a));
-    else
-        GTG_BY_SIZE(t.dtype, t.vocab, hipLaunchKernelGGL(HIP_KERNEL_NAME(distill_kernel<E, NT, false>), dim3((unsigned)t.rows), dim3(NT),
-                                                         lds, s, as_rows(t), a));
+                    Weight{gloss, gscale, norm, count ? t.rows : 0}, skip_unit ? 1 : 0, row_loss, dx, ldg};
+    const size_t lds = (size_t)((t.vocab + 16 + 31) / 32) * 4;
+    if (d.ce_weight != 0.0 && d.temperature != 1.0) {
+        by_size(t.dtype, t.vocab, [&](auto shape) {
+        typedef decltype(shape) P;
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(distill_kernel<typename P::E, P::NT, P::NV, true>), dim3((unsigned)t.rows), dim3(P::NT), lds, s, as_rows(t), a);
+    });
+    } else {
+        by_size(t.dtype, t.vocab, [&](auto shape) {
+        typedef decltype(shape) P;
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(distill_kernel<typename P::E, P::NT, P::NV, false>), dim3((unsigned)t.rows), dim3(P::NT), lds, s, as_rows(t), a);
+    });
+    }
     return check_launch("distill_kernel");
 }
 

@@ -702,22 +702,33 @@ def _need(ok, msg):
 
 
 def _token_rows(what, logits, targets):
-    """(logits as (rows, V) with unit stride along V, targets (rows) int64 contiguous): the tensors themselves where
-    their strides allow it, copies otherwise."""
-    _lib.require_cuda(logits, targets)
-    _need(logits.dtype in _DTYPES, f"{what}: logits must be float32, float16 or bfloat16, not {logits.dtype}")
-    _need(logits.dim() >= 1 and logits.shape[-1] >= 1, f"{what}: logits must be (..., vocab)")
-    x = logits if logits.dim() == 2 else logits.reshape(-1, logits.shape[-1])
-    if (x.stride(1) != 1 and x.shape[1] > 1) or (x.stride(0) < x.shape[1] and x.shape[0] > 1):
-        x = x.contiguous()
-    if targets is None:
-        return x, None
-    _need(targets.shape == logits.shape[:-1], f"{what}: targets {tuple(targets.shape)} do not match logits {tuple(logits.shape)}")
-    _same_device(what, x, targets)
-    _need(not (targets.is_floating_point() or targets.is_complex() or targets.dtype == torch.bool), f"{what}: targets must be integers")
-    if targets.dtype != torch.int64:
-        targets = targets.long()
-    return x, targets.contiguous()
+    """(x, y, (dtype code, rows, V, row stride)): the logits as memory of equally spaced rows with unit stride along V, and
+    the targets as contiguous int64 -- the tensors themselves where their strides allow it, copies otherwise."""
+    code = _DTYPES.get(logits.dtype)
+    if code is None or not logits.is_cuda:
+        _lib.require_cuda(logits, targets)
+        raise _lib.GtgError(f"{what}: logits must be float32, float16 or bfloat16, not {logits.dtype}")
+    shape = logits.shape
+    _need(len(shape) >= 1 and shape[-1] >= 1, f"{what}: logits must be (..., vocab)")
+    V = shape[-1]
+    R = logits.numel() // V
+    x, ld = logits, V
+    if not logits.is_contiguous():
+        x = logits if logits.dim() == 2 else logits.reshape(-1, V)
+        if (x.stride(1) != 1 and V > 1) or (x.stride(0) < V and R > 1):
+            x = x.contiguous()
+        elif R > 1:
+            ld = x.stride(0)
+    if targets is not None:
+        _lib.require_cuda(targets)
+        _need(targets.shape == shape[:-1], f"{what}: targets {tuple(targets.shape)} do not match logits {tuple(shape)}")
+        _same_device(what, x, targets)
+        if targets.dtype != torch.int64:
+            _need(not (targets.is_floating_point() or targets.is_complex() or targets.dtype == torch.bool),
+                  f"{what}: targets must be integers")
+            targets = targets.long()
+        targets = targets.contiguous()
+    return x, targets, (code, R, V, ld)
 
 
 def _same_device(what, x, *others):
@@ -730,36 +741,29 @@ def _row_floats(what, name, t, x, shape):
     """A float tensor of the rows' shape as contiguous fp32 on the logits' device."""
     _need(torch.is_tensor(t) and t.is_floating_point(), f"{what}: {name} must be a floating tensor")
     _same_device(what, x, t)
-    _need(tuple(t.shape) == tuple(shape), f"{what}: {name} must be {tuple(shape)}, not {tuple(t.shape)}")
-    return _f32c(t.detach())
+    _need(t.shape == shape, f"{what}: {name} must be {tuple(shape)}, not {tuple(t.shape)}")
+    return (t if t.dtype == torch.float32 else t.float()).contiguous()
 
 
 def _mask_bytes(what, mask, x, shape):
     if mask is None:
         return None
     _same_device(what, x, mask)
-    _need(tuple(mask.shape) == tuple(shape), f"{what}: mask must be {tuple(shape)}, not {tuple(mask.shape)}")
+    _need(mask.shape == shape, f"{what}: mask must be {tuple(shape)}, not {tuple(mask.shape)}")
     return (mask if mask.dtype == torch.bool else mask != 0).contiguous().view(torch.uint8)
 
 
-def _row_stride(x):
-    return x.stride(0) if x.shape[0] > 1 else max(x.stride(0), x.shape[1])
-
-
-def _grad_like(x):
-    """Uninitialised (rows, V) of x's type whose rows have x's rows' alignment modulo 16 bytes, so that the kernels
-    read and write whole 16-byte vectors; contiguous where x's rows allow that."""
-    R, V = x.shape
-    vec = 16 // x.element_size()
-    skew, off = (_row_stride(x) - V) % vec, x.data_ptr() % 16 // x.element_size()
+def _grad_like(x, shape, rows):
+    """(uninitialised gradient of the logits' shape and type, its row stride): its rows have the alignment of x's rows
+    modulo 16 bytes, so that the kernels read and write whole 16-byte vectors; contiguous where x's rows allow that."""
+    _, R, V, ld = rows
+    size = x.element_size()
+    vec = 16 // size
+    skew, off = (ld - V) % vec, x.data_ptr() % 16 // size
     if skew == 0 and off == 0:
-        return torch.empty((R, V), dtype=x.dtype, device=x.device)
+        return torch.empty(shape, dtype=x.dtype, device=x.device), V
     buf = torch.empty((R * (V + skew) + vec,), dtype=x.dtype, device=x.device)
-    return buf[off:off + R * (V + skew)].view(R, V + skew)[:, :V]
-
-
-def _logits_args(x):
-    return x.data_ptr(), _DTYPES[x.dtype], x.shape[0], x.shape[1], _row_stride(x)
+    return buf[off:off + R * (V + skew)].view(R, V + skew)[:, :V].view(shape), V + skew
 
 
 def _float_arg(what, name, v):
@@ -780,13 +784,13 @@ def top_logits(logits, k: int, temperature: float = 1.0):
     temperature) over the classes that were not selected (-inf where k == V).  1 <= k <= min(V, 256).  No gradient.
     What ``distill_loss`` takes of a teacher."""
     with torch.no_grad():
-        x, _ = _token_rows("top_logits", logits, None)
-        _need(isinstance(k, int) and 1 <= k <= min(256, x.shape[1]), "top_logits: k must be an integer in [1, min(vocab, 256)]")
+        x, _, rows = _token_rows("top_logits", logits, None)
+        _need(isinstance(k, int) and 1 <= k <= min(256, rows[2]), "top_logits: k must be an integer in [1, min(vocab, 256)]")
         lead = tuple(logits.shape[:-1])
         values = torch.empty(lead + (k,), dtype=x.dtype, device=x.device)
         indices = torch.empty(lead + (k,), dtype=torch.int32, device=x.device)
         tail = torch.empty(lead, dtype=torch.float32, device=x.device)
-        check(_lib.lib().gtg_top_logits(*_logits_args(x), k, _float_arg("top_logits", "temperature", temperature),
+        check(_lib.lib().gtg_top_logits(x.data_ptr(), *rows, k, _float_arg("top_logits", "temperature", temperature),
                                         values.data_ptr(), indices.data_ptr(), tail.data_ptr(), stream_ptr()), "gtg_top_logits")
     return values, indices, tail
 
@@ -798,15 +802,15 @@ class TokenLogprobFn(torch.autograd.Function):
     @staticmethod
     @_on_tensor_device
     def forward(ctx, logits, targets, padidx, temperature):
-        x, y = _token_rows("token_logprob", logits, targets)
+        x, y, rows = _token_rows("token_logprob", logits, targets)
         temperature = _float_arg("token_logprob", "temperature", temperature)
         logp = torch.empty(targets.shape, dtype=torch.float32, device=x.device)
         entropy = torch.empty_like(logp)
-        stats = torch.empty((x.shape[0], 4), dtype=torch.float32, device=x.device) if ctx.needs_input_grad[0] else None
-        check(_lib.lib().gtg_token_logprob_fwd(*_logits_args(x), y.data_ptr(), int(padidx), temperature, logp.data_ptr(),
+        stats = torch.empty((rows[1], 4), dtype=torch.float32, device=x.device) if ctx.needs_input_grad[0] else None
+        check(_lib.lib().gtg_token_logprob_fwd(x.data_ptr(), *rows, y.data_ptr(), int(padidx), temperature, logp.data_ptr(),
                                                entropy.data_ptr(), _opt(stats), stream_ptr()), "gtg_token_logprob_fwd")
         ctx.save_for_backward(x, y, stats)
-        ctx.key = (int(padidx), temperature, logits.shape)
+        ctx.key = (int(padidx), temperature, logits.shape, rows)
         ctx.set_materialize_grads(False)
         return logp, entropy
 
@@ -815,15 +819,15 @@ class TokenLogprobFn(torch.autograd.Function):
     @_on_tensor_device
     def backward(ctx, g_logp, g_entropy):
         x, y, stats = ctx.saved_tensors
-        padidx, temperature, shape = ctx.key
+        padidx, temperature, shape, rows = ctx.key
         if g_logp is None and g_entropy is None:
             return None, None, None, None
         g_logp, g_entropy = _f32c(g_logp), _f32c(g_entropy)
-        dx = _grad_like(x)
-        check(_lib.lib().gtg_token_logprob_bwd(*_logits_args(x), y.data_ptr(), padidx, temperature, stats.data_ptr(),
-                                               _opt(g_logp), _opt(g_entropy), dx.data_ptr(), _row_stride(dx), stream_ptr()),
+        dx, ldg = _grad_like(x, shape, rows)
+        check(_lib.lib().gtg_token_logprob_bwd(x.data_ptr(), *rows, y.data_ptr(), padidx, temperature, stats.data_ptr(),
+                                               _opt(g_logp), _opt(g_entropy), dx.data_ptr(), ldg, stream_ptr()),
               "gtg_token_logprob_bwd")
-        return dx.view(shape), None, None, None
+        return dx, None, None, None
 
 
 def token_logprob(logits, targets, padidx, temperature: float = 1.0):
@@ -842,41 +846,50 @@ class _RowLossFn(torch.autograd.Function):
     Without ``eager_grad``, and for reduction "none", the gradient is computed in the backward alone (two reads, one
     write).  A second backward through a retained graph computes it anew."""
 
-    # subclasses: _prepare(ctx, logits, *args) -> (x, saved tensors, reduction, eager_grad); _fwd / _bwd: the library call
+    # subclasses: OP, the entry points' name, and _args(saved tensors, key): what they take between logits and reduction
     @classmethod
-    def _run_forward(cls, ctx, op, x, shape, lead, saved, reduction, eager_grad, extra_outputs=0):
-        _need(reduction in _REDUCTIONS, f"{op}: reduction must be one of {sorted(_REDUCTIONS)}")
-        scalar = reduction != "none"
-        dev = x.device
-        row_loss = torch.empty(lead, dtype=torch.float32, device=dev)
-        loss = torch.empty((), dtype=torch.float32, device=dev) if scalar else None
-        norm = torch.empty((1,), dtype=torch.float64, device=dev) if reduction == "mean" else None
-        dx = _grad_like(x) if scalar and eager_grad and ctx.needs_input_grad[0] else None
-        extra = [torch.empty(lead, dtype=torch.float32, device=dev) for _ in range(extra_outputs)]
-        L = _lib.lib()
-        check(getattr(L, f"gtg_{op}_fwd")(*_logits_args(x), *cls._args(saved, ctx.key), _REDUCTIONS[reduction], _opt(norm),
-                                          row_loss.data_ptr(), _opt(loss), *[t.data_ptr() for t in extra], _opt(dx),
-                                          x.shape[1] if dx is None else _row_stride(dx), stream_ptr()), f"gtg_{op}_fwd")
-        ctx.save_for_backward(x, norm, *saved)
-        ctx.dx, ctx.scalar, ctx.shape = dx, scalar, shape
-        return (loss if scalar else row_loss), extra
+    def _run_forward(cls, ctx, x, rows, shape, lead, saved, reduction, eager_grad, outputs=()):
+        code = _REDUCTIONS.get(reduction)
+        _need(code is not None, f"{cls.OP}: reduction must be one of {sorted(_REDUCTIONS)}")
+        dev, R = x.device, rows[1]
+        dx, ldg = _grad_like(x, shape, rows) if code and eager_grad and ctx.needs_input_grad[0] else (None, rows[2])
+        if code:   # the mean's factor (8 bytes), then a loss per row
+            ws = torch.empty((R + 4,), dtype=torch.float32, device=dev)
+            loss = torch.empty((), dtype=torch.float32, device=dev)
+            norm, row_loss = ws.data_ptr() if code == 2 else None, ws.data_ptr() + 16
+        else:
+            ws, loss, norm = None, torch.empty(lead, dtype=torch.float32, device=dev), None
+            row_loss = loss.data_ptr()
+        rc = getattr(_lib.lib(), cls.FWD)(x.data_ptr(), *rows, *cls._args(saved, ctx.key), code, norm, row_loss,
+                                          loss.data_ptr() if code else None, *[t.data_ptr() for t in outputs],
+                                          None if dx is None else dx.data_ptr(), ldg, stream_ptr())
+        if rc:
+            check(rc, cls.FWD)
+        ctx.save_for_backward(x, ws, *saved)
+        ctx.dx, ctx.call = dx, (code, ldg, shape, rows)
+        return loss
 
     @classmethod
-    def _run_backward(cls, ctx, op, g):
-        x, norm, *saved = ctx.saved_tensors
+    def _run_backward(cls, ctx, g):
+        x, ws, *saved = ctx.saved_tensors
+        code, ldg, shape, rows = ctx.call
         g = _f32c(g)
         dx, ctx.dx = ctx.dx, None          # handed out once: afterwards it is the receiver's
         have = dx is not None
         if not have:
-            dx = _grad_like(x)
-        check(getattr(_lib.lib(), f"gtg_{op}_bwd")(*_logits_args(x), *cls._args(saved, ctx.key), _opt(norm),
-                                                   None if ctx.scalar else g.data_ptr(), g.data_ptr() if ctx.scalar else None,
-                                                   int(have), dx.data_ptr(), _row_stride(dx), stream_ptr()), f"gtg_{op}_bwd")
-        return dx.view(ctx.shape)
+            dx, ldg = _grad_like(x, shape, rows)
+        rc = getattr(_lib.lib(), cls.BWD)(x.data_ptr(), *rows, *cls._args(saved, ctx.key), ws.data_ptr() if code == 2 else None,
+                                          None if code else g.data_ptr(), g.data_ptr() if code else None, int(have),
+                                          dx.data_ptr(), ldg, stream_ptr())
+        if rc:
+            check(rc, cls.BWD)
+        return dx
 
 
 class DistillLossFn(_RowLossFn):
     """Loss of a student's logits against the classes a teacher lists; see distill_loss."""
+
+    OP, FWD, BWD = "distill_loss", "gtg_distill_loss_fwd", "gtg_distill_loss_bwd"
 
     @staticmethod
     def _args(saved, key):
@@ -889,28 +902,27 @@ class DistillLossFn(_RowLossFn):
     @_on_tensor_device
     def forward(ctx, logits, values, indices, targets, padidx, tail, temperature, ce_weight, reduction, eager_grad):
         what = "distill_loss"
-        x, y = _token_rows(what, logits, targets)
-        lead = tuple(targets.shape)
-        _need(values.dtype in _DTYPES and values.dim() == len(lead) + 1 and tuple(values.shape[:-1]) == lead and
-              1 <= values.shape[-1] <= 256, f"{what}: values must be {lead + ('k',)}, k in [1, 256], float32, float16 or bfloat16")
+        x, y, rows = _token_rows(what, logits, targets)
+        lead = targets.shape
+        _need(values.dtype in _DTYPES and values.dim() == len(lead) + 1 and values.shape[:-1] == lead and 1 <= values.shape[-1] <= 256,
+              f"{what}: values must be {tuple(lead) + ('k',)}, k in [1, 256], float32, float16 or bfloat16")
         _need(indices.dtype in (torch.int32, torch.int64) and indices.shape == values.shape,
               f"{what}: indices must be int32 or int64 of values' shape")
         _same_device(what, x, values, indices)
         if indices.dtype == torch.int64:
             # (what does not fit stays out of range, on its side)
             indices = indices.clamp(-1, 2 ** 31 - 1).int()
-        values, indices = values.detach().contiguous(), indices.contiguous()
+        values, indices = values.contiguous(), indices.contiguous()
         if tail is not None:
             tail = _row_floats(what, "tail", tail, x, lead)
         ctx.key = (int(padidx), _float_arg(what, "temperature", temperature), _float_arg(what, "ce_weight", ce_weight))
-        loss, _ = DistillLossFn._run_forward(ctx, what, x, logits.shape, lead, (y, values, indices, tail), reduction, eager_grad)
-        return loss
+        return DistillLossFn._run_forward(ctx, x, rows, logits.shape, lead, (y, values, indices, tail), reduction, eager_grad)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     @_on_tensor_device
     def backward(ctx, g):
-        return (DistillLossFn._run_backward(ctx, "distill_loss", g),) + (None,) * 9
+        return (DistillLossFn._run_backward(ctx, g),) + (None,) * 9
 
 
 def distill_loss(logits, values, indices, targets, padidx, tail=None, temperature: float = 1.0, ce_weight: float = 0.0,
@@ -934,6 +946,8 @@ def distill_loss(logits, values, indices, targets, padidx, tail=None, temperatur
 class PolicyLossFn(_RowLossFn):
     """Clipped policy loss with KL and entropy terms; see policy_loss."""
 
+    OP, FWD, BWD = "policy_loss", "gtg_policy_loss_fwd", "gtg_policy_loss_bwd"
+
     @staticmethod
     def _args(saved, key):
         y, old, adv, ref, mask = saved
@@ -945,11 +959,11 @@ class PolicyLossFn(_RowLossFn):
     def forward(ctx, logits, targets, padidx, old_logp, advantages, ref_logp, clip_low, clip_high, kl_coef, entropy_coef,
                 temperature, mask, reduction, eager_grad):
         what = "policy_loss"
-        x, y = _token_rows(what, logits, targets)
-        lead = tuple(targets.shape)
+        x, y, rows = _token_rows(what, logits, targets)
+        lead = targets.shape
         old = _row_floats(what, "old_logp", old_logp, x, lead)
         _need(torch.is_tensor(advantages), f"{what}: advantages must be a floating tensor")
-        per_column = len(lead) == 2 and tuple(advantages.shape) == lead[1:]
+        per_column = len(lead) == 2 and advantages.shape == lead[1:]
         adv = _row_floats(what, "advantages", advantages, x, lead[1:] if per_column else lead)
         ref = None if ref_logp is None else _row_floats(what, "ref_logp", ref_logp, x, lead)
         scalars = tuple(_float_arg(what, n, v) for n, v in (("clip_low", clip_low), ("clip_high", clip_high), ("kl_coef", kl_coef),
@@ -957,7 +971,9 @@ class PolicyLossFn(_RowLossFn):
         _need(scalars[2] == 0.0 or ref is not None, f"{what}: kl_coef needs ref_logp")
         ctx.key = (int(padidx), scalars)
         saved = (y, old, adv, ref, _mask_bytes(what, mask, x, lead))
-        loss, (logp, entropy) = PolicyLossFn._run_forward(ctx, what, x, logits.shape, lead, saved, reduction, eager_grad, 2)
+        logp = torch.empty(lead, dtype=torch.float32, device=x.device)
+        entropy = torch.empty_like(logp)
+        loss = PolicyLossFn._run_forward(ctx, x, rows, logits.shape, lead, saved, reduction, eager_grad, (logp, entropy))
         ctx.mark_non_differentiable(logp, entropy)
         ctx.set_materialize_grads(False)
         return loss, logp, entropy
@@ -966,7 +982,7 @@ class PolicyLossFn(_RowLossFn):
     @torch.autograd.function.once_differentiable
     @_on_tensor_device
     def backward(ctx, g, _glogp, _gentropy):
-        return (PolicyLossFn._run_backward(ctx, "policy_loss", g) if g is not None else None,) + (None,) * 13
+        return (PolicyLossFn._run_backward(ctx, g) if g is not None else None,) + (None,) * 13
 
 
 def policy_loss(logits, targets, padidx, old_logp, advantages, ref_logp=None, clip_low: float = 0.2, clip_high: float = 0.2,
@@ -994,26 +1010,30 @@ class PreferenceLossFn(torch.autograd.Function):
     @_on_tensor_device
     def forward(ctx, logits, targets, padidx, ref_logp, beta, label_smoothing, mask, batch_first, reduction):
         what = "preference_loss"
-        x, y = _token_rows(what, logits, targets)
+        x, y, rows = _token_rows(what, logits, targets)
         _need(targets.dim() == 2, f"{what}: targets must be (T, 2 P), or (2 P, T) with batch_first")
         _need(reduction in _REDUCTIONS, f"{what}: reduction must be one of {sorted(_REDUCTIONS)}")
-        S, T = targets.shape if batch_first else tuple(targets.shape)[::-1]
+        S, T = targets.shape if batch_first else targets.shape[::-1]
         _need(S % 2 == 0, f"{what}: an even number of sequences is needed, the chosen ones first, then the rejected ones")
         ref = _row_floats(what, "ref_logp", ref_logp, x, (S,))
         m = _mask_bytes(what, mask, x, targets.shape)
         beta, label_smoothing = _float_arg(what, "beta", beta), _float_arg(what, "label_smoothing", label_smoothing)
         L, dev, P = _lib.lib(), x.device, S // 2
-        empty = lambda *shape: torch.empty(shape, dtype=torch.float32, device=dev)  # noqa: E731
-        stats, coef, seq_logp, pair_loss = empty(x.shape[0], 4), empty(S), empty(S), empty(P)
-        loss = empty() if reduction != "none" else None
+        code, R, V, ld = rows
+        # for the backward: four numbers per row, one per sequence; here only: the call's workspace
+        state = torch.empty((4 * R + S,), dtype=torch.float32, device=dev)
+        seq_logp = torch.empty((S,), dtype=torch.float32, device=dev)
+        pair_loss = torch.empty((P,), dtype=torch.float32, device=dev)
+        loss = torch.empty((), dtype=torch.float32, device=dev) if reduction != "none" else None
         ws = _ws(L.gtg_preference_workspace_bytes(T, P), dev)
-        ptr_x, dtype, _, V, ld = _logits_args(x)
-        ctx.head = (dtype, T, P, V, ld, int(bool(batch_first)))
-        check(L.gtg_preference_fwd(ptr_x, *ctx.head, y.data_ptr(), int(padidx), _opt(m), ref.data_ptr(), beta, label_smoothing,
-                                   _REDUCTIONS[reduction], stats.data_ptr(), coef.data_ptr(), seq_logp.data_ptr(),
-                                   pair_loss.data_ptr(), _opt(loss), ws.data_ptr(), ws.numel(), stream_ptr()), "gtg_preference_fwd")
-        ctx.save_for_backward(x, y, m, stats, coef)
-        ctx.padidx, ctx.scalar, ctx.shape = int(padidx), loss is not None, logits.shape
+        ctx.head = (code, T, P, V, ld, int(bool(batch_first)))
+        rc = L.gtg_preference_fwd(x.data_ptr(), *ctx.head, y.data_ptr(), int(padidx), _opt(m), ref.data_ptr(), beta, label_smoothing,
+                                  _REDUCTIONS[reduction], state.data_ptr(), state.data_ptr() + 16 * R, seq_logp.data_ptr(),
+                                  pair_loss.data_ptr(), _opt(loss), ws.data_ptr(), ws.numel(), stream_ptr())
+        if rc:
+            check(rc, "gtg_preference_fwd")
+        ctx.save_for_backward(x, y, m, state)
+        ctx.padidx, ctx.scalar, ctx.shape, ctx.rows = int(padidx), loss is not None, logits.shape, rows
         ctx.mark_non_differentiable(seq_logp)
         ctx.set_materialize_grads(False)
         return (pair_loss if loss is None else loss), seq_logp
@@ -1024,14 +1044,15 @@ class PreferenceLossFn(torch.autograd.Function):
     def backward(ctx, g, _gseq):
         if g is None:
             return (None,) * 9
-        x, y, m, stats, coef = ctx.saved_tensors
+        x, y, m, state = ctx.saved_tensors
         g = _f32c(g)
-        dx = _grad_like(x)
-        check(_lib.lib().gtg_preference_bwd(x.data_ptr(), *ctx.head, y.data_ptr(), ctx.padidx, _opt(m), stats.data_ptr(),
-                                            coef.data_ptr(), g.data_ptr() if ctx.scalar else None,
-                                            None if ctx.scalar else g.data_ptr(), dx.data_ptr(), _row_stride(dx), stream_ptr()),
-              "gtg_preference_bwd")
-        return (dx.view(ctx.shape),) + (None,) * 8
+        dx, ldg = _grad_like(x, ctx.shape, ctx.rows)
+        rc = _lib.lib().gtg_preference_bwd(x.data_ptr(), *ctx.head, y.data_ptr(), ctx.padidx, _opt(m), state.data_ptr(),
+                                           state.data_ptr() + 16 * ctx.rows[1], g.data_ptr() if ctx.scalar else None,
+                                           None if ctx.scalar else g.data_ptr(), dx.data_ptr(), ldg, stream_ptr())
+        if rc:
+            check(rc, "gtg_preference_bwd")
+        return (dx,) + (None,) * 8
 
 
 def preference_loss(logits, targets, padidx, ref_logp, beta: float = 0.1, label_smoothing: float = 0.0, mask=None,
