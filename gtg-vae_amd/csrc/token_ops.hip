@@ -17,7 +17,7 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2v __attribute__((ext_vector_type(2)));
 
-constexpr double LOG2E = 1.4426950408889634;
+constexpr double LOG2E = 1.4426950408889634, LN2 = 0.6931471805599453;
 __device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
 // The hardware's 2^x: 1 step off at most, 0 where the result would lie below 2^-126.  The library's exp2f spends five more
 // instructions on those, as much again as everything else done per logit.
@@ -161,6 +161,20 @@ struct Row {
             if (bits[at >> 5] >> (at & 31) & 1) xe = neg_inf();
         }
     }
+    // f(value) in place of every value of the registers
+    template <typename F>
+    __device__ __forceinline__ void replace(F f)
+    {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            asm volatile("" : "+v"(v[k]));
+            float x[VEC];
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) x[q] = f(E::get(v[k], q));
+            v[k] = E::pack(x);
+        }
+        xe = f(xe);
+    }
     // f(index of the vector's first element, vector); ALL: also the places past the body's end, which hold -inf
     template <bool ALL, typename F>
     __device__ __forceinline__ void each(F f)
@@ -185,6 +199,14 @@ struct Row {
         }
     }
 };
+
+template <typename E>
+__device__ __forceinline__ float vec_max(float m, const u32x4& v)
+{
+#pragma unroll
+    for (int q = 0; q < E::VEC; ++q) m = fmaxf(m, E::get(v, q));
+    return m;
+}
 
 // A gradient row: vectors where its alignment is the logits' own, single elements otherwise.
 template <typename E>
@@ -219,64 +241,68 @@ __device__ __forceinline__ void fill_row(const R& row, const OutRow<E>& out, flo
 }
 
 // ---- reductions over a block ------------------------------------------------------------------------------------
-__device__ __forceinline__ float wave_max(float v)
+// Within a row of 16 lanes by DPP (two quad permutations and two mirrors: 4 instructions, no LDS), across the four rows by
+// reading one lane of each: the same bits in every lane.
+template <int CTRL>
+__device__ __forceinline__ int dpp(int v)
 {
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-    return v;
+    return __builtin_amdgcn_update_dpp(v, v, CTRL, 0xf, 0xf, true);
 }
-__device__ __forceinline__ float wave_sum(float v)
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v)
 {
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o);
-    return v;
+    return __int_as_float(dpp<CTRL>(__float_as_int(v)));
 }
-__device__ __forceinline__ double wave_sum(double v)
+template <int CTRL>
+__device__ __forceinline__ double dpp(double v)
 {
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o);
-    return v;
+    return __hiloint2double(dpp<CTRL>(__double2hiint(v)), dpp<CTRL>(__double2loint(v)));
+}
+__device__ __forceinline__ int lane_value(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+__device__ __forceinline__ float lane_value(float v, int lane) { return __int_as_float(lane_value(__float_as_int(v), lane)); }
+__device__ __forceinline__ double lane_value(double v, int lane)
+{
+    return __hiloint2double(lane_value(__double2hiint(v), lane), lane_value(__double2loint(v), lane));
+}
+template <typename T, typename F>
+__device__ __forceinline__ T wave_reduce(T v, F f)
+{
+    v = f(v, dpp<0xb1>(v));   // lanes 1 0 3 2 of every four
+    v = f(v, dpp<0x4e>(v));   // lanes 2 3 0 1
+    v = f(v, dpp<0x141>(v));  // every eight mirrored
+    v = f(v, dpp<0x140>(v));  // every sixteen mirrored
+    return f(f(lane_value(v, 0), lane_value(v, 16)), f(lane_value(v, 32), lane_value(v, 48)));
+}
+__device__ __forceinline__ float wave_max(float v) { return wave_reduce(v, [](float a, float b) { return fmaxf(a, b); }); }
+template <typename T>
+__device__ __forceinline__ T wave_sum(T v)
+{
+    return wave_reduce(v, [](T a, T b) { return a + b; });
 }
 
-template <int NT>
+// Over the block, through one place of LDS per wave.  AGAIN: the places may still be read from an earlier call.
+template <int NT, bool AGAIN, typename T, typename F>
+__device__ __forceinline__ T block_reduce(T v, T* sh, F f)
+{
+    v = wave_reduce(v, f);
+    if (NT == 64) return v;
+    if (AGAIN) __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = sh[0];
+#pragma unroll
+    for (int w = 1; w < NT / 64; ++w) v = f(v, sh[w]);
+    return v;
+}
+template <int NT, bool AGAIN>
 __device__ __forceinline__ float block_max(float v, float* sh)
 {
-    v = wave_max(v);
-    if (NT == 64) return v;
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = sh[0];
-#pragma unroll
-    for (int w = 1; w < NT / 64; ++w) v = fmaxf(v, sh[w]);
-    return v;
+    return block_reduce<NT, AGAIN>(v, sh, [](float a, float b) { return fmaxf(a, b); });
 }
-template <int NT>
-__device__ __forceinline__ float block_sum(float v, float* sh)
+template <int NT, bool AGAIN, typename T>
+__device__ __forceinline__ T block_sum(T v, T* sh)
 {
-    v = wave_sum(v);
-    if (NT == 64) return v;
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = sh[0];
-#pragma unroll
-    for (int w = 1; w < NT / 64; ++w) v += sh[w];
-    return v;
-}
-template <int NT>
-__device__ __forceinline__ int block_count(int v, int* sh)
-{
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o);
-    if (NT == 64) return v;
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = sh[0];
-#pragma unroll
-    for (int w = 1; w < NT / 64; ++w) v += sh[w];
-    return v;
+    return block_reduce<NT, AGAIN>(v, sh, [](T a, T b) { return a + b; });
 }
 
 // ---- exponential and logarithm in 64 bits, for one number per row --------------------------------------------------
@@ -324,8 +350,6 @@ __device__ __forceinline__ double log_row(double x)
     const double l = fma((double)e, 0.69314718055994531, 2.0 * z * p);
     return x == 0.0 ? -__builtin_inf() : x == __builtin_inf() ? x : l;
 }
-__device__ __forceinline__ double from_lane(double v, int lane) { return __shfl(v, lane); }
-
 __device__ __forceinline__ float finite_or_zero(float m) { return m == neg_inf() ? 0.f : m; }
 // x - m, from below at the lowest finite number: its product with exp(-inf) = 0 is then 0 and not NaN
 __device__ __forceinline__ float clamped(float d) { return fmaxf(d, -3.402823466e38f); }
@@ -362,7 +386,7 @@ __device__ __forceinline__ double mean_norm(const Rows& rows, const Weight& w, i
     if (w.count == 0) return w.norm ? *w.norm : 1.0;
     int n = 0;
     for (int r = threadIdx.x; r < (int)w.count; r += NT) n += rows.kept(r) ? 1 : 0;
-    n = block_count<NT>(n, sh);
+    n = block_sum<NT, true>(n, sh);
     const double norm = n > 0 ? 1.0 / (double)n : 0.0;
     if (blockIdx.x == 0 && threadIdx.x == 0) *w.norm = norm;
     return norm;
@@ -374,7 +398,7 @@ __global__ __launch_bounds__(1024) void count_kernel(Rows rows, int64_t R, doubl
     __shared__ int sh[16];
     int n = 0;
     for (int64_t r = threadIdx.x; r < R; r += 1024) n += rows.kept(r) ? 1 : 0;
-    n = block_count<1024>(n, sh);
+    n = block_sum<1024, false>(n, sh);
     if (threadIdx.x == 0) *norm = n > 0 ? 1.0 / (double)n : 0.0;
 }
 
@@ -396,105 +420,154 @@ __global__ __launch_bounds__(1024) void total_kernel(const float* __restrict__ r
 }
 
 // ---- maximum, sum of exponentials and a second sum -----------------------------------------------------------------
-// m = max x, s = sum exp2(c (x - m)), and by KIND a second sum: MOMENT: t = sum exp2(c (x - m)) (x - m), TWO: t = sum
-// exp2(c1 (x - m)), NONE.  All of the row, in every thread.  Each thread finds them for its own elements -- the maximum
-// first where they are in registers, all in one sweep with a running maximum where they are not -- and one reduction over
-// the block joins them; differences are taken before the scaling so that the type's lowest value in every place is a row
-// like any other.
-enum Second { NONE, MOMENT, TWO };
-template <Second KIND>
-struct Stats {
-    float m = -__builtin_inff(), s = 0.f, t = 0.f;
-
-    // to the maximum M >= m
-    __device__ __forceinline__ void raise(float M, float c, float c1)
+// A logit's place below the row's maximum m is taken in powers of two with one rounding: y = x c - mu, c = log2(e) / tau
+// and mu = m c, both rounded; 2^y is within 2^-24 |y| + 2^-23 of the exact power, and a sum of them is read relative to mu.
+// mu's own rounding is a common factor of 2^(m c - mu).  Where mu is so large that this is no small one (logits of a million,
+// masks of the type's lowest value in all places) the row is made flat first: x - m takes the place of x, mu is 0.
+struct Scale {
+    float c, mu, m;
+    bool flat;
+    __device__ __forceinline__ Scale(float m_, float c_) : c(c_), m(m_)
     {
-        if (m == neg_inf()) {
-            s = t = 0.f;
-        } else {
-            const float d = m - M, f = exp2_raw(d * c);
-            if (KIND == MOMENT) t = f == 0.f ? 0.f : f * (t + d * s);  // (d s may be infinite where f is 0)
-            if (KIND == TWO) t *= exp2_raw(d * c1);
-            s *= f;
-        }
-        m = M;
+        mu = m * c;
+        flat = m != neg_inf() && m != __builtin_inff() && !(fabsf(mu) < 1048576.f);
+        if (flat || m == neg_inf()) mu = 0.f;
     }
-    // me: m, or 0 where m is -inf
-    __device__ __forceinline__ void add(float x, float me, float c, float c1)
+    __device__ __forceinline__ void make_flat()
     {
-        const float d = x - me, e = exp2_raw(d * c);
-        s += e;
-        if (KIND == MOMENT) t += e * clamped(d);
-        if (KIND == TWO) t += exp2_raw(d * c1);
+        flat = true;
+        mu = 0.f;
+    }
+    __device__ __forceinline__ float y(float x) const { return fmaf(x, c, -mu); }
+    // in 64 bits and units of e: the log of a logit's exponential relative to the sums' reference
+    __device__ __forceinline__ double log_of(float x, double inv_tau) const
+    {
+        return flat ? ((double)x - (double)m) * inv_tau : fma((double)x, (double)c, -(double)mu) * LN2;
+    }
+    // the sums' own reference relative to another logit `to`, likewise
+    __device__ __forceinline__ double log_ref(float to, double inv_tau) const
+    {
+        if (m == neg_inf()) return -__builtin_inf();
+        return flat ? ((double)m - (double)to) * inv_tau : fma(-(double)to, (double)c, (double)mu) * LN2;
+    }
+    // this reference minus another's, in powers of two
+    __device__ __forceinline__ float above(const Scale& o) const
+    {
+        if (flat) return o.flat ? (m - o.m) * c : fmaf(m, c, -o.mu);
+        return o.flat ? fmaf(-o.m, c, mu) : mu - o.mu;
     }
 };
 
+// s = sum 2^y and by KIND a second sum: MOMENT: t = sum 2^y y; TWO: t = sum 2^y1 by a second scale; NONE.
+enum Second { NONE, MOMENT, TWO };
+struct Stats {
+    float s = 0.f, t = 0.f;
+    template <Second KIND>
+    __device__ __forceinline__ void add(float x, const Scale& a, const Scale& b)
+    {
+        const float y = a.y(x), e = exp2_raw(y);
+        s += e;
+        if (KIND == MOMENT) t = fmaf(e, clamped(y), t);
+        if (KIND == TWO) t += exp2_raw(b.y(x));
+    }
+};
+
+// Every thread gets the row's m (in a and b) and sums.  Rows in registers: the maximum of the whole row first, then the
+// sums.  Rows read again in every sweep: one sweep for both, each thread relative to the largest logit it has met, joined at
+// the end.  sh: 3 x 16 places.
 template <Second KIND, typename E, int NT, int NV, bool MARKED>
-__device__ __forceinline__ Stats<KIND> row_stats(Row<E, NT, NV, MARKED>& row, float c, float c1, float* sh)
+__device__ __forceinline__ Stats row_stats(Row<E, NT, NV, MARKED>& row, float c, float c1, Scale& a, Scale& b, float* sh)
 {
-    Stats<KIND> a;
-    a.m = row.xe;
+    Stats r;
     if constexpr (NV > 0) {
+        float m = neg_inf();
+        row.template each<true>([&](int, const u32x4& v) { m = vec_max<E>(m, v); });
+        m = block_max<NT, false>(fmaxf(m, row.xe), sh);
+        a = Scale(m, c);
+        b = Scale(m, c1);
+        if (a.flat || (KIND == TWO && b.flat)) {
+            if (m != neg_inf()) row.replace([&](float x) { return x - m; });
+            a.make_flat();
+            b.make_flat();
+        }
         row.template each<true>([&](int, const u32x4& v) {
 #pragma unroll
-            for (int q = 0; q < E::VEC; ++q) a.m = fmaxf(a.m, E::get(v, q));
+            for (int q = 0; q < E::VEC; ++q) r.add<KIND>(E::get(v, q), a, b);
         });
-        const float me = finite_or_zero(a.m);
-        a.add(row.xe, me, c, c1);
-        row.template each<true>([&](int, const u32x4& v) {
-#pragma unroll
-            for (int q = 0; q < E::VEC; ++q) a.add(E::get(v, q), me, c, c1);
-        });
+        r.add<KIND>(row.xe, a, b);
     } else {
-        a.add(row.xe, finite_or_zero(a.m), c, c1);
+        float m = row.xe;
+        auto start = [&](float M) {
+            a = Scale(M, c);
+            b = Scale(M, c1);
+            if (KIND == TWO && (a.flat || b.flat)) {
+                a.make_flat();
+                b.make_flat();
+            }
+        };
+        start(m);
+        auto raise = [&](float M) {  // the sums so far to the maximum M > m
+            const Scale o = a, o1 = b;
+            start(M);
+            const float d = o.m == neg_inf() ? neg_inf() : o.above(a), f = exp2_raw(d);
+            if (KIND == MOMENT) r.t = f == 0.f ? 0.f : f * (r.t + d * r.s);
+            if (KIND == TWO) r.t *= o.m == neg_inf() ? 0.f : exp2_raw(o1.above(b));
+            r.s *= f;  // (0 of a sum without terms; a NaN stays)
+            m = M;
+        };
+        if (m != neg_inf()) r.add<KIND>(a.flat ? 0.f : m, a, b);
         row.template each<true>([&](int, const u32x4& v) {
-            float vm = E::get(v, 0);
+            const float vm = vec_max<E>(neg_inf(), v);
+            if (vm > m) raise(vm);
 #pragma unroll
-            for (int q = 1; q < E::VEC; ++q) vm = fmaxf(vm, E::get(v, q));
-            if (vm > a.m) a.raise(vm, c, c1);
-            const float me = finite_or_zero(a.m);
-#pragma unroll
-            for (int q = 0; q < E::VEC; ++q) a.add(E::get(v, q), me, c, c1);
+            for (int q = 0; q < E::VEC; ++q) {
+                const float x = E::get(v, q);
+                r.add<KIND>(a.flat ? x - m : x, a, b);
+            }
         });
+        const float M = block_max<NT, false>(m, sh);
+        if (M > m) raise(M);
     }
-    // (the sums are needed on one side of raise()'s branch only: without this they are moved there, sweep and all)
-    asm volatile("" : "+v"(a.s), "+v"(a.t));
-    a.raise(wave_max(a.m), c, c1);
-    a.s = wave_sum(a.s);
-    if (KIND != NONE) a.t = wave_sum(a.t);
-    if (NT > 64) {
-        constexpr int NW = NT / 64;
-        const int w = threadIdx.x >> 6;
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) {
-            sh[w] = a.m;
-            sh[NW + w] = a.s;
-            if (KIND != NONE) sh[2 * NW + w] = a.t;
-        }
-        __syncthreads();
-        float M = sh[0];
+    // (kept from moving the sums, sweep and all, to where they are used)
+    asm volatile("" : "+v"(r.s), "+v"(r.t));
+    if (NT > 64) sh += 16;
+    r.s = block_sum<NT, false>(r.s, sh);
+    if (NT > 64) sh += 16;
+    if (KIND != NONE) r.t = block_sum<NT, false>(r.t, sh);
+    if (r.s == __builtin_inff()) r.s = __builtin_nanf("");
+    return r;
+}
+
+// The gradient's sweep: grad(logit) for every one, gy more at class `target` (-1: none).  FLATTEN: the row's vectors hold
+// logits as they stand in memory and the scale wants them flat.
+template <bool FLATTEN, typename R, typename E, typename F>
+__device__ __forceinline__ void store_sweep(R& row, const OutRow<E>& out, const Scale& a, int target, float gy, F grad)
+{
+    auto value = [&](float x) { return grad(FLATTEN ? x - a.m : x); };
+    row.template each<false>([&](int j, const u32x4& v) {
+        float f[E::VEC];
 #pragma unroll
-        for (int i = 1; i < NW; ++i) M = fmaxf(M, sh[i]);
-        Stats<KIND> all;
-        all.m = M;
+        for (int q = 0; q < E::VEC; ++q) f[q] = value(E::get(v, q));
+        if ((unsigned)(target - j) < (unsigned)E::VEC) {
 #pragma unroll
-        for (int i = 0; i < NW; ++i) {
-            Stats<KIND> b;
-            b.m = sh[i];
-            b.s = sh[NW + i];
-            b.t = KIND != NONE ? sh[2 * NW + i] : 0.f;
-            b.raise(M, c, c1);
-            all.s += b.s;
-            all.t += b.t;
+            for (int q = 0; q < E::VEC; ++q)
+                if (target == j + q) f[q] += gy;
         }
-        a = all;
-    }
-    return a;
+        out.vec(j, f);
+    });
+    if (row.je >= 0) out.one(row.je, value(row.xe) + (row.je == target ? gy : 0.f));
+}
+template <bool HELD, typename R, typename E, typename F>
+__device__ __forceinline__ void store_row(R& row, const OutRow<E>& out, const Scale& a, int target, float gy, F grad)
+{
+    // (rows held in registers are flat already where the scale is)
+    if (!HELD && a.flat) store_sweep<true>(row, out, a, target, gy, grad);
+    else store_sweep<false>(row, out, a, target, gy, grad);
 }
 
 // ---- log-probability and entropy ---------------------------------------------------------------------------------
-// logp = x_y / tau - lse, entropy = log s - t / (s tau).  stats (R, 4): m, 1 / s, -t / (s tau), unused: what the
-// backward needs.  logp64 (R): the log-probability unrounded, for the sums of the preference loss.
+// logp = (x_y - m) / tau - log s, entropy H = log s + u, u = -ln 2 t / s.  stats (R, 4): m, 1 / s, u, unused: what the backward
+// needs.  logp64 (R): the log-probability unrounded, for the sums of the preference loss.
 struct LogprobOut {
     float* logp;
     float* entropy;
@@ -518,20 +591,20 @@ __global__ __launch_bounds__(NT, min_waves(NV)) void logprob_kernel(Rows rows, d
     const typename E::Store* x = reinterpret_cast<const typename E::Store*>(rows.x) + r * rows.ld;
     Row<E, NT, NV> row(x, rows.vocab);
     row.load();
-    const Stats<MOMENT> a = row_stats<MOMENT>(row, (float)(LOG2E * inv_tau), 0.f, sh);
+    Scale sc(neg_inf(), 0.f), unused(neg_inf(), 0.f);
+    const Stats a = row_stats<MOMENT>(row, (float)(LOG2E * inv_tau), 0.f, sc, unused, sh);
     if (threadIdx.x == 0) {
-        const float m = finite_or_zero(a.m), s = a.s, t = a.t;
         const int64_t y = rows.targets[r];
-        const double log_s = log_row((double)s), u = -(double)t / (double)s * inv_tau;
-        const double lp = (y >= 0 && y < rows.vocab) ? ((double)E::load(x + y) - (double)m) * inv_tau - log_s : __builtin_nan("");
+        const double log_s = log_row((double)a.s), u = -(double)a.t / (double)a.s * LN2;
+        const double lp = (y >= 0 && y < rows.vocab) ? sc.log_of(E::load(x + y), inv_tau) - log_s : __builtin_nan("");
         if (out.logp) out.logp[r] = (float)lp;
         if (out.entropy) out.entropy[r] = (float)(log_s + u);
         if (out.logp64) out.logp64[r] = lp;
-        if (out.stats) out.stats[r] = make_float4(m, 1.f / s, (float)u, 0.f);
+        if (out.stats) out.stats[r] = make_float4(sc.m, 1.f / a.s, (float)u, 0.f);
     }
 }
 
-// d/dx_j = (1/tau) [ g_l (1[j = y] - p_j) - g_H p_j (log p_j + H) ],  log p_j + H = (x_j - m) / tau + u
+// d/dx_j = (1/tau) [ g_l (1[j = y] - p_j) - g_H p_j (log p_j + H) ],  log p_j + H = ln 2 y_j + u
 // The coefficients g_l are one per row, or one per sequence: group 0: g_l[r], S > 0: g_l[r mod S] (time-major),
 // S < 0: g_l[r / -S] (sequence by sequence).
 struct RowGrad {
@@ -569,21 +642,14 @@ __global__ __launch_bounds__(NT) void logprob_bwd_kernel(Rows rows, RowGrad g)
     if (bad) gl = __builtin_nanf("");
     const float4 st = g.stats[r];
     const float gh = g.g_entropy ? g.g_entropy[r] : 0.f;
-    const float c = (float)(LOG2E * g.inv_tau), it = (float)g.inv_tau, m = st.x;
-    // exp(c (x - m)) (k0 + k1 (x - m)) + [j = y] gy
-    const float gy = gl * it, k0 = -(gl + gh * st.z) * it * st.y, k1 = -gh * it * it * st.y;
-    auto value = [&](int j, float xv) {
-        const float d = xv - m;
-        float v = exp2_raw(d * c) * (k0 + k1 * clamped(d));
-        return j == y ? v + gy : v;
-    };
-    row.template each<false>([&](int j, const u32x4& v) {
-        float f[E::VEC];
-#pragma unroll
-        for (int q = 0; q < E::VEC; ++q) f[q] = value(j + q, E::get(v, q));
-        out.vec(j, f);
+    const Scale a(st.x, (float)(LOG2E * g.inv_tau));
+    // 2^y (k0 + k1 y) + [j = target] gy
+    const float it = (float)g.inv_tau, gy = gl * it, k0 = -(gl + gh * st.z) * it * st.y, k1 = -gh * it * st.y * (float)LN2;
+    if (k1 == 0.f) store_row<false>(row, out, a, y, gy, [&](float v) { return exp2_raw(a.y(v)) * k0; });
+    else store_row<false>(row, out, a, y, gy, [&](float v) {
+        const float e = a.y(v);
+        return exp2_raw(e) * fmaf(k1, clamped(e), k0);
     });
-    if (row.je >= 0) out.one(row.je, value(row.je, row.xe));
 }
 
 // ---- clipped policy loss -------------------------------------------------------------------------------------------
@@ -625,18 +691,18 @@ __global__ __launch_bounds__(NT, min_waves(NV)) void policy_kernel(Rows rows, Po
         return;
     }
     row.load();
-    const float c = (float)(LOG2E * a.inv_tau);
-    const Stats<MOMENT> all = row_stats<MOMENT>(row, c, 0.f, sh);
-    const float m = finite_or_zero(all.m), s = all.s, t = all.t;
+    Scale sc(neg_inf(), 0.f), unused(neg_inf(), 0.f);
+    const Stats all = row_stats<MOMENT>(row, (float)(LOG2E * a.inv_tau), 0.f, sc, unused, sh);
+    const float s = all.s, t = all.t;
     const int64_t y64 = rows.targets[r];
     const int y = (y64 >= 0 && y64 < rows.vocab) ? (int)y64 : -1;
     if (threadIdx.x < 64) {
-        const double it = a.inv_tau, log_s = log_row((double)s), u = -(double)t / (double)s * it, H = log_s + u;
-        const double lp = y >= 0 ? ((double)E::load(x + y) - (double)m) * it - log_s : __builtin_nan("");
+        const double it = a.inv_tau, log_s = log_row((double)s), u = -(double)t / (double)s * LN2, H = log_s + u;
+        const double lp = y >= 0 ? sc.log_of(E::load(x + y), it) - log_s : __builtin_nan("");
         const double A = (double)a.adv[r % a.adv_rows], gap = a.ref_logp ? (double)a.ref_logp[r] - lp : 0.0;
         // two exponentials, side by side in two lanes
         const double both = exp_row(threadIdx.x == 0 ? lp - (double)a.old_logp[r] : gap);
-        const double rho = from_lane(both, 0), away = from_lane(both, 1);
+        const double rho = lane_value(both, 0), away = lane_value(both, 1);
         const double free = rho * A, held = (rho < a.lo ? a.lo : rho > a.hi ? a.hi : rho) * A;
         double loss = free <= held ? -free : -held, g = free <= held ? -free : 0.0;
         if (free != free) loss = g = free;  // a NaN stays one
@@ -651,25 +717,18 @@ __global__ __launch_bounds__(NT, min_waves(NV)) void policy_kernel(Rows rows, Po
             if (a.entropy) a.entropy[r] = (float)H;
             const double w = a.w.of(r, norm) * it;
             coef[0] = (float)(w * (-g + a.ent * u) / (double)s);
-            coef[1] = (float)(w * a.ent * it / (double)s);
+            coef[1] = (float)(w * a.ent * LN2 / (double)s);
             coef[2] = (float)(w * g);
         }
     }
     if (!a.dx) return;
     __syncthreads();
     const float k0 = coef[0], k1 = coef[1], gy = coef[2];
-    auto value = [&](int j, float xv) {
-        const float d = xv - m;
-        float v = exp2_raw(d * c) * (k0 + k1 * clamped(d));
-        return j == y ? v + gy : v;
-    };
-    row.template each<false>([&](int j, const u32x4& v) {
-        float f[E::VEC];
-#pragma unroll
-        for (int q = 0; q < E::VEC; ++q) f[q] = value(j + q, E::get(v, q));
-        out.vec(j, f);
+    if (k1 == 0.f) store_row<(NV > 0)>(row, out, sc, y, gy, [&](float v) { return exp2_raw(sc.y(v)) * k0; });
+    else store_row<(NV > 0)>(row, out, sc, y, gy, [&](float v) {
+        const float e = sc.y(v);
+        return exp2_raw(e) * fmaf(k1, clamped(e), k0);
     });
-    if (row.je >= 0) out.one(row.je, value(row.je, row.xe));
 }
 
 // ---- distillation from a teacher's list of logits ----------------------------------------------------------------
@@ -773,8 +832,9 @@ __global__ __launch_bounds__(NT, min_waves(NV)) void distill_kernel(Rows rows, D
 
     // the classes outside the list: maximum, sums at both temperatures
     const float c = (float)(LOG2E * a.inv_tau), c1 = (float)LOG2E;
-    const auto rest = row_stats<BOTH ? TWO : NONE>(row, c, c1, sh);
-    const float m_rest = rest.m, mt = finite_or_zero(rest.m), s_tau = rest.s, s_one = BOTH ? rest.t : rest.s;
+    Scale sc(neg_inf(), c), sc1(neg_inf(), c1);
+    const Stats rest = row_stats<BOTH ? TWO : NONE>(row, c, c1, sc, sc1, sh);
+    const float m_rest = sc.m, s_tau = rest.s, s_one = BOTH ? rest.t : rest.s;
 
     // one wave: the teacher's distribution, the student's sums over everything, the loss
     if (tid < 64) {
@@ -806,15 +866,15 @@ __global__ __launch_bounds__(NT, min_waves(NV)) void distill_kernel(Rows rows, D
         s1 = BOTH ? wave_sum(s1) : 0.0;
         cross = wave_sum(cross);
         // exponentials and logarithms side by side in the wave's lanes; those that scale every class outside the list,
-        // of (the others' maximum) - (the row's), in 64 bits like the rest
-        const double gap = (double)m_rest - (double)m;
-        const double e3 = exp_row(tid == 0 ? tail - M : tid == 1 ? gap * it : gap);
-        const double qt0 = from_lane(e3, 0), lift = from_lane(e3, 1), lift1 = BOTH ? from_lane(e3, 2) : lift;
+        // of (the others' reference) - (the row's maximum), in 64 bits like the rest
+        const double gap = sc.log_ref(m, it), gap1 = BOTH ? sc1.log_ref(m, 1.0) : gap;
+        const double e3 = exp_row(tid == 0 ? tail - M : tid == 1 ? gap : gap1);
+        const double qt0 = lane_value(e3, 0), lift = lane_value(e3, 1), lift1 = BOTH ? lane_value(e3, 2) : lift;
         z += qt0;
         s += (double)s_tau * lift;
         s1 = BOTH ? s1 + (double)s_one * lift1 : s;
         const double l4 = log_row(tid == 0 ? z : tid == 1 ? s : tid == 2 ? (double)s_tau : s1);
-        const double log_z = from_lane(l4, 0), log_s = from_lane(l4, 1), log_rest = from_lane(l4, 2), log_s1 = from_lane(l4, 3);
+        const double log_z = lane_value(l4, 0), log_s = lane_value(l4, 1), log_rest = lane_value(l4, 2), log_s1 = lane_value(l4, 3);
         const bool none = z == 0.0;  // the teacher says nothing about this row
         const double qt = none ? 0.0 : qt0 / z;
         double kd = 0.0;
@@ -822,7 +882,7 @@ __global__ __launch_bounds__(NT, min_waves(NV)) void distill_kernel(Rows rows, D
         if (!none && wkd != 0.0) {
             // everything relative to the two maxima M and m, which may be as large as the type's lowest value
             kd = cross / z - (log_z - log_s);
-            if (qt != 0.0) kd += qt * ((tail - M) - (log_rest + gap * it));
+            if (qt != 0.0) kd += qt * ((tail - M) - (log_rest + gap));
             kd *= wkd * a.tau * a.tau;
         }
         double ce = 0.0;
@@ -846,19 +906,10 @@ __global__ __launch_bounds__(NT, min_waves(NV)) void distill_kernel(Rows rows, D
     if (!a.dx) return;
     __syncthreads();
     const float ka = coef[0], kb = coef[1], gy = coef[2];
-    auto value = [&](int j, float xv) {
-        const float d = xv - mt;
-        float v = exp2_raw(d * c) * ka;
-        if (BOTH) v += exp2_raw(d * c1) * kb;
-        return j == y ? v - gy : v;
-    };
-    row.template each<false>([&](int j, const u32x4& v) {
-        float f[E::VEC];
-#pragma unroll
-        for (int q = 0; q < E::VEC; ++q) f[q] = value(j + q, E::get(v, q));
-        out.vec(j, f);
+    store_row<(NV > 0)>(row, out, sc, y, -gy, [&](float v) {
+        const float e = exp2_raw(sc.y(v)) * ka;
+        return BOTH ? fmaf(exp2_raw(sc1.y(v)), kb, e) : e;
     });
-    if (row.je >= 0) out.one(row.je, value(row.je, row.xe));
     __syncthreads();  // the listed classes' gradients go over what the row's vectors left in their places
     for (int k = tid; k < a.k; k += NT) {
         if (!own[k]) continue;
@@ -883,11 +934,11 @@ __device__ __forceinline__ unsigned order_key(float x)
     return x != x ? 0xffffffffu : (b & 0x80000000u) ? ~b : b | 0x80000000u;
 }
 
-// The usual way takes two sweeps.  The first finds every thread's two maxima (over the vectors' halves): the k-th largest
-// of those, 2 NT numbers, is a bound that at least k elements reach and, for k well below 2 NT, few more do.  The second
-// puts what reaches the bound on a list and sums the exponentials of everything below, relative to the bound.  The list's
-// elements then find their rank by comparing with each other.  Where the list would overflow (many equal values), or a
-// NaN is about, the k-th largest is found bit by bit with a sweep for each; where what lies below the bound vanishes
+// The usual way takes two sweeps.  The first finds maxima of parts of the row, one per thread (two, over the vectors' halves,
+// for a k that is not small beside the threads): the k-th largest of them is a bound that at least k elements reach and few
+// more do.  The second puts what reaches the bound on a list and sums the exponentials of everything below, relative to
+// the bound.  The list's elements then find their rank by comparing with each other.  Where the list would overflow (many equal
+// values), or a NaN is about, the k-th largest is found bit by bit with a sweep for each; where what lies below the bound vanishes
 // beside it, the tail is summed in two more sweeps relative to its own maximum.
 constexpr int TOP_LIST = 1024;
 
@@ -896,20 +947,49 @@ __device__ __forceinline__ float key_value(unsigned key)  // the float of a key 
     return __uint_as_float((key & 0x80000000u) ? key ^ 0x80000000u : ~key);
 }
 
+// One wave: the k-th largest of the n keys (a multiple of 64, at most 64 N), to 16 bits and rounded down.  The bits above the
+// highest one in which any two keys differ are common to all.
+template <int N>
+__device__ __forceinline__ unsigned kth_key16(const unsigned* keys, int n, int k)
+{
+    unsigned mk[N], all_or = 0, all_and = 0xffffffffu;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        mk[i] = 64 * i < n ? keys[(threadIdx.x & 63) + 64 * i] : 0;
+        if (64 * i < n) {
+            all_or |= mk[i];
+            all_and &= mk[i];
+        }
+    }
+    const unsigned differ = (unsigned)wave_reduce((int)all_or, [](int a, int b) { return a | b; }) ^
+                            (unsigned)wave_reduce((int)all_and, [](int a, int b) { return a & b; });
+    const int top = differ ? 31 - __builtin_clz(differ) : -1;
+    unsigned kth = top >= 31 ? 0u : (unsigned)lane_value((int)all_and, 0) & (0xffffffffu << (top + 1));
+#pragma unroll 1
+    for (int bit = top; bit >= 16; --bit) {
+        const unsigned cand = kth | (1u << bit);
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (64 * i < n) c += __popcll(__ballot(mk[i] >= cand));
+        if (c >= k) kth = cand;
+    }
+    return kth & 0xffff0000u;
+}
+
 template <typename E, int NT, int NV>
 __global__ __launch_bounds__(NT, min_waves(NV)) void top_kernel(const void* logits, int64_t ld, int V, int k, double inv_tau,
-                                                 void* __restrict__ values, int32_t* __restrict__ indices,
-                                                 float* __restrict__ tail)
+                                                                void* __restrict__ values, int32_t* __restrict__ indices,
+                                                                float* __restrict__ tail)
 {
     __shared__ float shf[16];
     __shared__ int sh[16];
     __shared__ int fill;
     __shared__ unsigned bound_key, kth_key;
     __shared__ int kth_idx;
-    __shared__ unsigned ckey[TOP_LIST];
-    __shared__ int cidx[TOP_LIST];
-    __shared__ float rest[TOP_LIST];     // listed but not among the k, in order
-    __shared__ unsigned maxima[2 * NT];
+    __shared__ unsigned long long list[TOP_LIST];  // key, then the complement of the index: larger is nearer the front
+    __shared__ int ranks[TOP_LIST];
+    __shared__ unsigned keys[2 * NT];              // maxima; then the floats that are listed but not among the k, in order
     const int64_t r = blockIdx.x;
     const int tid = threadIdx.x;
     const typename E::Store* x = reinterpret_cast<const typename E::Store*>(logits) + r * ld;
@@ -917,7 +997,8 @@ __global__ __launch_bounds__(NT, min_waves(NV)) void top_kernel(const void* logi
     row.load();
     const float c = (float)(LOG2E * inv_tau);
 
-    float lo = row.xe, hi = neg_inf();
+    const bool halves = 4 * k > NT;
+    float lo = neg_inf(), hi = neg_inf();
     row.template each<true>([&](int, const u32x4& v) {
 #pragma unroll
         for (int q = 0; q < E::VEC / 2; ++q) {
@@ -925,59 +1006,48 @@ __global__ __launch_bounds__(NT, min_waves(NV)) void top_kernel(const void* logi
             hi = fmaxf(hi, E::get(v, q + E::VEC / 2));
         }
     });
-    maxima[tid] = order_key(lo);
-    maxima[NT + tid] = order_key(hi);
+    lo = fmaxf(lo, row.xe);
+    keys[tid] = order_key(halves ? lo : fmaxf(lo, hi));
+    if (halves) keys[NT + tid] = order_key(hi);
     if (tid == 0) fill = 0;
+    for (int i = tid; i < TOP_LIST; i += NT) ranks[i] = 0;
     __syncthreads();
     if (tid < 64) {
-        // the k-th largest maximum to 16 bits, rounded down
-        unsigned mk[2 * NT / 64];
-#pragma unroll
-        for (int i = 0; i < 2 * NT / 64; ++i) mk[i] = maxima[tid + 64 * i];
-        unsigned kth = 0;
-#pragma unroll 1
-        for (unsigned bit = 0x80000000u; bit >= 0x10000u; bit >>= 1) {
-            const unsigned cand = kth | bit;
-            int n = 0;
-#pragma unroll
-            for (int i = 0; i < 2 * NT / 64; ++i) n += __popcll(__ballot(mk[i] >= cand));
-            if (n >= k) kth = cand;
-        }
-        if (tid == 0) bound_key = kth;
+        const unsigned key = halves ? kth_key16<2 * NT / 64>(keys, 2 * NT, k) : kth_key16<NT / 64>(keys, NT, k);
+        if (tid == 0) bound_key = key;
     }
     __syncthreads();
     const float bound = bound_key > order_key(neg_inf()) ? key_value(bound_key) : neg_inf();
-    auto put = [&](int j, float f) {
-        const int at = atomicAdd(&fill, 1);
-        if (at < TOP_LIST) {
-            ckey[at] = order_key(f);
-            cidx[at] = j;
-        }
+    auto put = [&](int at, int j, float f) {
+        if (at < TOP_LIST) list[at] = (unsigned long long)order_key(f) << 32 | (unsigned)~j;
     };
+    const Scale sc(bound, c);
     float s = 0.f;
-    auto below = [&](float f) { s += exp2_raw((f - bound) * c); };
-    if (row.je >= 0) {
-        if (row.xe < bound) below(row.xe);
-        else put(row.je, row.xe);
-    }
-    row.template each<false>([&](int j, const u32x4& v) {
-        float vm = E::get(v, 0);
+    row.template each<false>([&](int j, u32x4& v) {
+        const float vm = vec_max<E>(neg_inf(), v);
+        if (!(vm < bound)) {
+            int n = 0;
 #pragma unroll
-        for (int q = 1; q < E::VEC; ++q) vm = fmaxf(vm, E::get(v, q));
-        if (vm < bound) {
-#pragma unroll
-            for (int q = 0; q < E::VEC; ++q) below(E::get(v, q));  // (a NaN among them shows in the sum)
-        } else {
+            for (int q = 0; q < E::VEC; ++q) n += !(E::get(v, q) < bound) ? 1 : 0;
+            int at = atomicAdd(&fill, n);
 #pragma unroll
             for (int q = 0; q < E::VEC; ++q) {
                 const float f = E::get(v, q);
-                if (f < bound) below(f);
-                else put(j + q, f);
+                if (!(f < bound)) {
+                    put(at++, j + q, f);
+                    E::clear(v, q);
+                }
             }
         }
+#pragma unroll
+        for (int q = 0; q < E::VEC; ++q) s += exp2_raw(sc.y(E::get(v, q)));  // (a NaN that vm passed over shows in the sum)
     });
-    s = block_sum<NT>(s, shf);
-    __syncthreads();
+    if (row.je >= 0) {
+        if (row.xe < bound) s += exp2_raw(sc.y(row.xe));
+        else put(atomicAdd(&fill, 1), row.je, row.xe);
+    }
+    s = block_sum<NT, false>(s, shf);
+    if (NT == 64) __syncthreads();
     int n = fill;
     const bool exact = n > TOP_LIST || s != s;
     Row<E, NT, 0> again(x, V);  // the rare ways read the row anew: their loops need no registers of the usual one's
@@ -989,7 +1059,7 @@ __global__ __launch_bounds__(NT, min_waves(NV)) void top_kernel(const void* logi
 #pragma unroll
                 for (int q = 0; q < E::VEC; ++q) cnt += pred(j + q, E::get(v, q)) ? 1 : 0;
             });
-            return block_count<NT>(cnt, sh);
+            return block_sum<NT, true>(cnt, sh);
         };
         unsigned kth = 0;  // the largest key that at least k elements reach
         for (int bit = 31; bit >= 0; --bit) {
@@ -1007,7 +1077,7 @@ __global__ __launch_bounds__(NT, min_waves(NV)) void top_kernel(const void* logi
         __syncthreads();
         auto take = [&](int j, float f) {
             const unsigned key = order_key(f);
-            if (key > kth || (key == kth && j <= last)) put(j, f);
+            if (key > kth || (key == kth && j <= last)) put(atomicAdd(&fill, 1), j, f);
         };
         if (again.je >= 0) take(again.je, again.xe);
         again.template each<false>([&](int j, const u32x4& v) {
@@ -1017,38 +1087,50 @@ __global__ __launch_bounds__(NT, min_waves(NV)) void top_kernel(const void* logi
         __syncthreads();
         n = k;
     }
-    for (int i = tid; i < n; i += NT) {
-        const unsigned ki = ckey[i];
-        const int ji = cidx[i];
-        int rank = 0;
-        for (int o = 0; o < n; ++o) rank += ckey[o] > ki || (ckey[o] == ki && cidx[o] < ji) ? 1 : 0;
-        if (rank < k) {
-            indices[r * k + rank] = ji;
-            reinterpret_cast<typename E::Store*>(values)[r * k + rank] = x[ji];
-            if (rank == k - 1) {
-                kth_key = ki;
-                kth_idx = ji;
-            }
-        } else {
-            rest[rank - k] = key_value(ki);
+    // ranks: a wave compares 64 of the list's elements with its share of the whole list
+    {
+        constexpr int NW = NT / 64;
+        const int w = tid >> 6, lane = tid & 63;
+        const int share = (n + NW - 1) / NW, o0 = w * share, o1 = min(n, o0 + share);
+        for (int i0 = 0; i0 < n; i0 += 64) {
+            const unsigned long long mine = list[min(i0 + lane, n - 1)];
+            int rank = 0;
+#pragma unroll 4
+            for (int o = o0; o < o1; ++o) rank += list[o] > mine ? 1 : 0;
+            if (i0 + lane < n && rank) atomicAdd(&ranks[i0 + lane], rank);
         }
     }
     __syncthreads();
-    if (!exact && (s > 1e-30f || n == V)) {
+    float* rest = reinterpret_cast<float*>(keys);
+    const bool spare = n - k <= 2 * NT;  // (the maxima's places hold what is listed beyond k; more than they are goes the long way)
+    for (int i = tid; i < n; i += NT) {
+        const unsigned key = (unsigned)(list[i] >> 32);
+        const int j = (int)~(unsigned)list[i], rank = ranks[i];
+        if (rank < k) {
+            indices[r * k + rank] = j;
+            reinterpret_cast<typename E::Store*>(values)[r * k + rank] = x[j];
+            if (rank == k - 1) {
+                kth_key = key;
+                kth_idx = j;
+            }
+        } else if (spare) {
+            rest[rank - k] = key_value(key);
+        }
+    }
+    __syncthreads();
+    if (!exact && spare && !sc.flat && (s > 1e-30f || n == V)) {
         // what lies below the bound, and the list's own remainder relative to its first
         if (tid < 64) {
             const float first = n > k ? rest[0] : neg_inf();
             float t = 0.f;
             for (int i = tid; i < n - k; i += 64) t += first == neg_inf() ? 0.f : exp2_raw((rest[i] - first) * c);
             t = wave_sum(t);
-            if (tid == 0) {
-                const double top = fmax((double)first, s > 0.f ? (double)bound : (double)neg_inf());
-                double sum = 0.0;
-                if (s > 0.f) sum += (double)s * exp_row(((double)bound - top) * inv_tau);
-                if (t > 0.f) sum += (double)t * exp_row(((double)first - top) * inv_tau);
-                // (an infinite first, and a NaN, which is before every number, are the sum themselves)
-                tail[r] = first == __builtin_inff() || first != first ? first : sum > 0.0 ? (float)(top * inv_tau + log_row(sum)) : neg_inf();
-            }
+            const double low = s > 0.f ? (double)sc.mu * LN2 : (double)neg_inf(), high = (double)first * inv_tau;
+            const double top = fmax(low, high);
+            const double e = exp_row(tid == 0 ? low - top : high - top);
+            const double sum = (s > 0.f ? (double)s * lane_value(e, 0) : 0.0) + (t > 0.f ? (double)t * lane_value(e, 1) : 0.0);
+            // (an infinite first, and a NaN, which is before every number, are the sum themselves)
+            if (tid == 0) tail[r] = first == __builtin_inff() || first != first ? first : sum > 0.0 ? (float)(top + log_row(sum)) : neg_inf();
         }
         return;
     }
@@ -1067,7 +1149,7 @@ __global__ __launch_bounds__(NT, min_waves(NV)) void top_kernel(const void* logi
             if (!chosen(j + q, f)) mx = fmaxf(mx, f);
         }
     });
-    const float m_rest = block_max<NT>(mx, shf), m = finite_or_zero(m_rest);
+    const float m_rest = block_max<NT, true>(mx, shf), m = finite_or_zero(m_rest);
     s = again.je >= 0 && !chosen(again.je, again.xe) ? exp2_raw((again.xe - m) * c) : 0.f;
     again.template each<false>([&](int j, const u32x4& v) {
 #pragma unroll
@@ -1076,7 +1158,7 @@ __global__ __launch_bounds__(NT, min_waves(NV)) void top_kernel(const void* logi
             if (!chosen(j + q, f)) s += exp2_raw((f - m) * c);
         }
     });
-    s = block_sum<NT>(s, shf);
+    s = block_sum<NT, true>(s, shf);
     if (tid == 0) tail[r] = m_rest == __builtin_inff() && s != s ? m_rest : (float)(log_row((double)s) + (double)m * inv_tau);
 }
 
