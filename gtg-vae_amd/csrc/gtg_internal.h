@@ -385,12 +385,12 @@ bool counts_in_rows(int64_t R);
 int count_rows(const TokenRows& t, double* norm, hipStream_t s);
 int total_loss(const float* row_loss, int64_t R, const double* norm, float* loss, hipStream_t s);
 // row r's gradient is weighted with gloss[r] * *gscale * *norm (each 1 where NULL); count: *norm is found here;
-// skip_unit: the launch does nothing where *gscale is 1
+// unless_unit: the launch does nothing where *gscale is 1
 int policy_rows(const TokenRows& t, const PolicyRows& p, const float* gloss, const float* gscale, double* norm, bool count,
-                bool skip_unit, float* row_loss, float* logp, float* entropy, void* dx, int64_t ldg, hipStream_t s);
+                bool unless_unit, float* row_loss, float* logp, float* entropy, void* dx, int64_t ldg, hipStream_t s);
 int distill_max_vocab();
 int distill_rows(const TokenRows& t, const DistillRows& d, const float* gloss, const float* gscale, double* norm, bool count,
-                 bool skip_unit, float* row_loss, void* dx, int64_t ldg, hipStream_t s);
+                 bool unless_unit, float* row_loss, void* dx, int64_t ldg, hipStream_t s);
 int prefer_pairs(const double* logp, double* seq, int64_t T, int64_t pairs, bool batch_first, const float* ref, double beta,
                  double label_smoothing, bool mean, float* seq_logp, float* coef, float* pair_loss, float* loss,
                  hipStream_t s);

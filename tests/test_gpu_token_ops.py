@@ -639,6 +639,36 @@ def test_offsets_past_32_bits():
     assert torch.equal(i[rows].cpu(), O.top_logits(some, 8)[1])
 
 
+def test_more_rows_than_one_launch_takes():
+    """2^21 rows go into one launch; the rows behind them into the next."""
+    R, V = (1 << 21) + 5000, 3
+    g = torch.Generator().manual_seed(2)
+    x = torch.randn((R, V), generator=g)
+    y = torch.randint(0, 3, (R,), generator=g)
+    f = 0.1 * torch.randn((R,), generator=g)
+    xg = x.cuda().requires_grad_(True)
+    x64 = x.double().requires_grad_(True)
+    loss, logp, ent = _fn().policy_loss(xg, y.cuda(), 0, f.cuda() - 1.0, f.cuda(), entropy_coef=0.1)
+    rows, wl, we = O.policy_rows(x64, y, 0, f - 1.0, f, entropy_coef=0.1)
+    want = O.reduce(rows, y != 0, "mean")
+    delta, D = _delta(x)
+    _check_rows(logp, wl.detach(), delta)
+    _check_rows(ent, we.detach(), delta * (D + 2))
+    assert abs(loss.item() - want.item()) < 1e-6
+    (got,) = torch.autograd.grad(loss, (xg,))
+    (w,) = torch.autograd.grad(want, x64)
+    _check_grad(got, w, torch.full((R, 1), 2.0 / int((y != 0).sum())) * (D + 2), delta)
+    logp, _ = _fn().token_logprob(xg, y.cuda(), 0)
+    (got,) = torch.autograd.grad(logp.sum(), (xg,))
+    p = torch.softmax(x.double(), -1)
+    want = torch.where((y != 0)[:, None], torch.nn.functional.one_hot(y, 3) - p, 0.0)
+    _check_grad(got, want, torch.ones(R, 1), delta)
+    v, i, t = _fn().top_logits(xg, 2)
+    assert torch.equal(i.cpu().long(), torch.topk(x, 2).indices)
+    loss = _fn().distill_loss(xg, v, i, y.cuda(), 0, t, reduction="none")
+    assert loss.abs().max().item() < 1e-5 and loss.shape == (R,)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_strided_logits_and_a_gradient_of_another_alignment(dtype):
     Fn = _fn()
