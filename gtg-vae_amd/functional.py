@@ -19,11 +19,13 @@ def _on_tensor_device(fn):
     current device is another GPU."""
     @functools.wraps(fn)
     def wrapped(*args, **kwargs):
-        dev = next((a.device for a in args if torch.is_tensor(a) and a.is_cuda), None)
-        if dev is None or dev.index == torch.cuda.current_device():
-            return fn(*args, **kwargs)
-        with torch.cuda.device(dev):
-            return fn(*args, **kwargs)
+        for a in args:
+            if isinstance(a, torch.Tensor) and a.is_cuda:
+                if a.device.index == torch.cuda.current_device():
+                    break
+                with torch.cuda.device(a.device):
+                    return fn(*args, **kwargs)
+        return fn(*args, **kwargs)
     return wrapped
 
 
@@ -783,16 +785,40 @@ def top_logits(logits, k: int, temperature: float = 1.0):
     Returns (values (..., k) of the logits' type, indices (..., k) int32, tail (...) fp32), tail = log sum exp(logits /
     temperature) over the classes that were not selected (-inf where k == V).  1 <= k <= min(V, 256).  No gradient.
     What ``distill_loss`` takes of a teacher."""
-    with torch.no_grad():
-        x, _, rows = _token_rows("top_logits", logits, None)
-        _need(isinstance(k, int) and 1 <= k <= min(256, rows[2]), "top_logits: k must be an integer in [1, min(vocab, 256)]")
-        lead = tuple(logits.shape[:-1])
-        values = torch.empty(lead + (k,), dtype=x.dtype, device=x.device)
-        indices = torch.empty(lead + (k,), dtype=torch.int32, device=x.device)
-        tail = torch.empty(lead, dtype=torch.float32, device=x.device)
-        check(_lib.lib().gtg_top_logits(x.data_ptr(), *rows, k, _float_arg("top_logits", "temperature", temperature),
-                                        values.data_ptr(), indices.data_ptr(), tail.data_ptr(), stream_ptr()), "gtg_top_logits")
+    x, _, rows = _token_rows("top_logits", logits.detach() if logits.requires_grad else logits, None)
+    _need(isinstance(k, int) and 1 <= k <= min(256, rows[2]), "top_logits: k must be an integer in [1, min(vocab, 256)]")
+    lead, dev = logits.shape[:-1], x.device
+    values = torch.empty(lead + (k,), dtype=x.dtype, device=dev)
+    indices = torch.empty(lead + (k,), dtype=torch.int32, device=dev)
+    tail = torch.empty(lead, dtype=torch.float32, device=dev)
+    rc = _lib.lib().gtg_top_logits(x.data_ptr(), *rows, k, _float_arg("top_logits", "temperature", temperature), values.data_ptr(),
+                                   indices.data_ptr(), tail.data_ptr(), stream_ptr())
+    if rc:
+        check(rc, "gtg_top_logits")
     return values, indices, tail
+
+
+def _grad_wanted(logits):
+    """Whether a call records a gradient: without one the library is called past autograd (4 us less per call)."""
+    return torch.is_grad_enabled() and logits.requires_grad
+
+
+# The autograd functions below take the logits and one plain tuple with everything else (tensors among it, which get no
+# gradient): autograd looks at every argument of a call, and a call on a small batch lasts no longer than that.
+
+
+@_on_tensor_device
+def _token_logprob(logits, targets, padidx, temperature, stats_too):
+    x, y, rows = _token_rows("token_logprob", logits, targets)
+    temperature = _float_arg("token_logprob", "temperature", temperature)
+    logp = torch.empty(targets.shape, dtype=torch.float32, device=x.device)
+    entropy = torch.empty_like(logp)
+    stats = torch.empty((rows[1], 4), dtype=torch.float32, device=x.device) if stats_too else None
+    rc = _lib.lib().gtg_token_logprob_fwd(x.data_ptr(), *rows, y.data_ptr(), int(padidx), temperature, logp.data_ptr(),
+                                          entropy.data_ptr(), _opt(stats), stream_ptr())
+    if rc:
+        check(rc, "gtg_token_logprob_fwd")
+    return logp, entropy, (x, y, stats), (int(padidx), temperature, logits.shape, rows)
 
 
 class TokenLogprobFn(torch.autograd.Function):
@@ -800,17 +826,9 @@ class TokenLogprobFn(torch.autograd.Function):
     padidx; both differentiable.  The backward reads the logits once more and keeps four numbers per row."""
 
     @staticmethod
-    @_on_tensor_device
-    def forward(ctx, logits, targets, padidx, temperature):
-        x, y, rows = _token_rows("token_logprob", logits, targets)
-        temperature = _float_arg("token_logprob", "temperature", temperature)
-        logp = torch.empty(targets.shape, dtype=torch.float32, device=x.device)
-        entropy = torch.empty_like(logp)
-        stats = torch.empty((rows[1], 4), dtype=torch.float32, device=x.device) if ctx.needs_input_grad[0] else None
-        check(_lib.lib().gtg_token_logprob_fwd(x.data_ptr(), *rows, y.data_ptr(), int(padidx), temperature, logp.data_ptr(),
-                                               entropy.data_ptr(), _opt(stats), stream_ptr()), "gtg_token_logprob_fwd")
-        ctx.save_for_backward(x, y, stats)
-        ctx.key = (int(padidx), temperature, logits.shape, rows)
+    def forward(ctx, logits, args):
+        logp, entropy, saved, ctx.key = _token_logprob(logits, *args, True)
+        ctx.save_for_backward(*saved)
         ctx.set_materialize_grads(False)
         return logp, entropy
 
@@ -818,26 +836,55 @@ class TokenLogprobFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     @_on_tensor_device
     def backward(ctx, g_logp, g_entropy):
+        if g_logp is None and g_entropy is None:
+            return None, None
         x, y, stats = ctx.saved_tensors
         padidx, temperature, shape, rows = ctx.key
-        if g_logp is None and g_entropy is None:
-            return None, None, None, None
         g_logp, g_entropy = _f32c(g_logp), _f32c(g_entropy)
         dx, ldg = _grad_like(x, shape, rows)
-        check(_lib.lib().gtg_token_logprob_bwd(x.data_ptr(), *rows, y.data_ptr(), padidx, temperature, stats.data_ptr(),
-                                               _opt(g_logp), _opt(g_entropy), dx.data_ptr(), ldg, stream_ptr()),
-              "gtg_token_logprob_bwd")
-        return dx, None, None, None
+        rc = _lib.lib().gtg_token_logprob_bwd(x.data_ptr(), *rows, y.data_ptr(), padidx, temperature, stats.data_ptr(), _opt(g_logp),
+                                              _opt(g_entropy), dx.data_ptr(), ldg, stream_ptr())
+        if rc:
+            check(rc, "gtg_token_logprob_bwd")
+        return dx, None
 
 
 def token_logprob(logits, targets, padidx, temperature: float = 1.0):
     """(logp, entropy), each of targets' shape: log softmax(logits / temperature) at the target and the entropy of that
     distribution; logits (..., V) fp32, fp16 or bf16, targets (...) integers.  Rows whose target is padidx give zero, a
     target outside the vocabulary NaN.  See TokenLogprobFn."""
-    return TokenLogprobFn.apply(logits, targets, padidx, temperature)
+    if _grad_wanted(logits):
+        return TokenLogprobFn.apply(logits, (targets, padidx, temperature))
+    return _token_logprob(logits, targets, padidx, temperature, False)[:2]
 
 
-class _RowLossFn(torch.autograd.Function):
+@_on_tensor_device
+def _row_loss_fwd(logits, op, args, reduction, with_grad):
+    """The forward of a row loss (`op`: _DistillLoss or _PolicyLoss): (outputs, tensors for the backward, the gradient for an
+    upstream gradient of 1 or None, the rest for the backward)."""
+    x, y, rows = _token_rows(op.NAME, logits, args[0])
+    code = _REDUCTIONS.get(reduction)
+    _need(code is not None, f"{op.NAME}: reduction must be one of {sorted(_REDUCTIONS)}")
+    saved, scalars = op.check(x, args)
+    lead, shape, dev = args[0].shape, logits.shape, x.device
+    dx, ldg = _grad_like(x, shape, rows) if code and with_grad else (None, rows[2])
+    if code:   # the mean's factor (8 bytes), then a loss per row
+        ws = torch.empty((rows[1] + 4,), dtype=torch.float32, device=dev)
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        at = ws.data_ptr()
+        norm, row_loss, total = at if code == 2 else None, at + 16, loss.data_ptr()
+    else:
+        ws, loss, norm, total = None, torch.empty(lead, dtype=torch.float32, device=dev), None, None
+        row_loss = loss.data_ptr()
+    outputs = (loss,) + op.outputs(lead, dev)
+    rc = op.fwd()(x.data_ptr(), *rows, y.data_ptr(), *op.pointers(saved, scalars), code, norm, row_loss, total,
+                  *[t.data_ptr() for t in outputs[1:]], None if dx is None else dx.data_ptr(), ldg, stream_ptr())
+    if rc:
+        check(rc, op.NAME)
+    return outputs, (x, y, ws) + saved, dx, (op, scalars, code, ldg, shape, rows)
+
+
+class RowLossFn(torch.autograd.Function):
     """What the distillation and the policy loss share: a loss per row of logits and its gradient from one sweep.
 
     With a scalar reduction and ``eager_grad`` the forward writes the logits' gradient for an upstream gradient of 1
@@ -846,83 +893,71 @@ class _RowLossFn(torch.autograd.Function):
     Without ``eager_grad``, and for reduction "none", the gradient is computed in the backward alone (two reads, one
     write).  A second backward through a retained graph computes it anew."""
 
-    # subclasses: OP, the entry points' name, and _args(saved tensors, key): what they take between logits and reduction
-    @classmethod
-    def _run_forward(cls, ctx, x, rows, shape, lead, saved, reduction, eager_grad, outputs=()):
-        code = _REDUCTIONS.get(reduction)
-        _need(code is not None, f"{cls.OP}: reduction must be one of {sorted(_REDUCTIONS)}")
-        dev, R = x.device, rows[1]
-        dx, ldg = _grad_like(x, shape, rows) if code and eager_grad and ctx.needs_input_grad[0] else (None, rows[2])
-        if code:   # the mean's factor (8 bytes), then a loss per row
-            ws = torch.empty((R + 4,), dtype=torch.float32, device=dev)
-            loss = torch.empty((), dtype=torch.float32, device=dev)
-            norm, row_loss = ws.data_ptr() if code == 2 else None, ws.data_ptr() + 16
-        else:
-            ws, loss, norm = None, torch.empty(lead, dtype=torch.float32, device=dev), None
-            row_loss = loss.data_ptr()
-        rc = getattr(_lib.lib(), cls.FWD)(x.data_ptr(), *rows, *cls._args(saved, ctx.key), code, norm, row_loss,
-                                          loss.data_ptr() if code else None, *[t.data_ptr() for t in outputs],
-                                          None if dx is None else dx.data_ptr(), ldg, stream_ptr())
-        if rc:
-            check(rc, cls.FWD)
-        ctx.save_for_backward(x, ws, *saved)
-        ctx.dx, ctx.call = dx, (code, ldg, shape, rows)
-        return loss
+    @staticmethod
+    def forward(ctx, logits, call):
+        outputs, saved, ctx.dx, ctx.rest = _row_loss_fwd(logits, *call)
+        ctx.save_for_backward(*saved)
+        if len(outputs) == 1:
+            return outputs[0]
+        ctx.mark_non_differentiable(*outputs[1:])
+        ctx.set_materialize_grads(False)
+        return outputs
 
-    @classmethod
-    def _run_backward(cls, ctx, g):
-        x, ws, *saved = ctx.saved_tensors
-        code, ldg, shape, rows = ctx.call
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    @_on_tensor_device
+    def backward(ctx, g, *_):
+        if g is None:
+            return None, None
+        x, y, ws, *saved = ctx.saved_tensors
+        op, scalars, code, ldg, shape, rows = ctx.rest
         g = _f32c(g)
         dx, ctx.dx = ctx.dx, None          # handed out once: afterwards it is the receiver's
         have = dx is not None
         if not have:
             dx, ldg = _grad_like(x, shape, rows)
-        rc = getattr(_lib.lib(), cls.BWD)(x.data_ptr(), *rows, *cls._args(saved, ctx.key), ws.data_ptr() if code == 2 else None,
-                                          None if code else g.data_ptr(), g.data_ptr() if code else None, int(have),
-                                          dx.data_ptr(), ldg, stream_ptr())
+        rc = op.bwd()(x.data_ptr(), *rows, y.data_ptr(), *op.pointers(saved, scalars), ws.data_ptr() if code == 2 else None,
+                      None if code else g.data_ptr(), g.data_ptr() if code else None, int(have), dx.data_ptr(), ldg, stream_ptr())
         if rc:
-            check(rc, cls.BWD)
-        return dx
+            check(rc, op.NAME)
+        return dx, None
 
 
-class DistillLossFn(_RowLossFn):
-    """Loss of a student's logits against the classes a teacher lists; see distill_loss."""
+class _DistillLoss:
+    """distill_loss's part of RowLossFn; args: (targets, values, indices, padidx, tail, temperature, ce_weight)."""
 
-    OP, FWD, BWD = "distill_loss", "gtg_distill_loss_fwd", "gtg_distill_loss_bwd"
-
-    @staticmethod
-    def _args(saved, key):
-        y, values, indices, tail = saved
-        padidx, temperature, ce_weight = key
-        return (y.data_ptr(), padidx, values.data_ptr(), _DTYPES[values.dtype], indices.data_ptr(), values.shape[-1], _opt(tail),
-                temperature, ce_weight)
+    NAME = "distill_loss"
+    fwd = staticmethod(lambda: _lib.lib().gtg_distill_loss_fwd)
+    bwd = staticmethod(lambda: _lib.lib().gtg_distill_loss_bwd)
 
     @staticmethod
-    @_on_tensor_device
-    def forward(ctx, logits, values, indices, targets, padidx, tail, temperature, ce_weight, reduction, eager_grad):
+    def check(x, args):
         what = "distill_loss"
-        x, y, rows = _token_rows(what, logits, targets)
-        lead = targets.shape
-        _need(values.dtype in _DTYPES and values.dim() == len(lead) + 1 and values.shape[:-1] == lead and 1 <= values.shape[-1] <= 256,
+        targets, values, indices, padidx, tail, temperature, ce_weight = args
+        lead, shape = targets.shape, values.shape
+        _need(values.dtype in _DTYPES and len(shape) == len(lead) + 1 and shape[:-1] == lead and 1 <= shape[-1] <= 256,
               f"{what}: values must be {tuple(lead) + ('k',)}, k in [1, 256], float32, float16 or bfloat16")
-        _need(indices.dtype in (torch.int32, torch.int64) and indices.shape == values.shape,
+        _need(indices.dtype in (torch.int32, torch.int64) and indices.shape == shape,
               f"{what}: indices must be int32 or int64 of values' shape")
         _same_device(what, x, values, indices)
         if indices.dtype == torch.int64:
             # (what does not fit stays out of range, on its side)
             indices = indices.clamp(-1, 2 ** 31 - 1).int()
-        values, indices = values.contiguous(), indices.contiguous()
         if tail is not None:
             tail = _row_floats(what, "tail", tail, x, lead)
-        ctx.key = (int(padidx), _float_arg(what, "temperature", temperature), _float_arg(what, "ce_weight", ce_weight))
-        return DistillLossFn._run_forward(ctx, x, rows, logits.shape, lead, (y, values, indices, tail), reduction, eager_grad)
+        return ((values.contiguous(), indices.contiguous(), tail),
+                (int(padidx), _float_arg(what, "temperature", temperature), _float_arg(what, "ce_weight", ce_weight)))
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    @_on_tensor_device
-    def backward(ctx, g):
-        return (DistillLossFn._run_backward(ctx, g),) + (None,) * 9
+    def outputs(lead, dev):
+        return ()
+
+    @staticmethod
+    def pointers(saved, scalars):
+        values, indices, tail = saved
+        padidx, temperature, ce_weight = scalars
+        return (padidx, values.data_ptr(), _DTYPES[values.dtype], indices.data_ptr(), values.shape[-1],
+                None if tail is None else tail.data_ptr(), temperature, ce_weight)
 
 
 def distill_loss(logits, values, indices, targets, padidx, tail=None, temperature: float = 1.0, ce_weight: float = 0.0,
@@ -939,50 +974,47 @@ def distill_loss(logits, values, indices, targets, padidx, tail=None, temperatur
 
     reduction: "mean" over the rows that count (0 if there are none), "sum", or "none" (a loss per row).  Differentiable
     in the logits alone.  ``eager_grad=False`` for a scalar loss that will be scaled before its backward -- by a gradient
-    scaler, a number of accumulation steps -- : the gradient is then computed in the backward only, see _RowLossFn."""
-    return DistillLossFn.apply(logits, values, indices, targets, padidx, tail, temperature, ce_weight, reduction, eager_grad)
+    scaler, a number of accumulation steps -- : the gradient is then computed in the backward only, see RowLossFn."""
+    args = (targets, values, indices, padidx, tail, temperature, ce_weight)
+    if _grad_wanted(logits):
+        return RowLossFn.apply(logits, (_DistillLoss, args, reduction, eager_grad))
+    return _row_loss_fwd(logits, _DistillLoss, args, reduction, False)[0][0]
 
 
-class PolicyLossFn(_RowLossFn):
-    """Clipped policy loss with KL and entropy terms; see policy_loss."""
+class _PolicyLoss:
+    """policy_loss's part of RowLossFn; args: (targets, padidx, old_logp, advantages, ref_logp, mask, clip_low, clip_high,
+    kl_coef, entropy_coef, temperature)."""
 
-    OP, FWD, BWD = "policy_loss", "gtg_policy_loss_fwd", "gtg_policy_loss_bwd"
+    NAME = "policy_loss"
+    fwd = staticmethod(lambda: _lib.lib().gtg_policy_loss_fwd)
+    bwd = staticmethod(lambda: _lib.lib().gtg_policy_loss_bwd)
+    NUMBERS = ("clip_low", "clip_high", "kl_coef", "entropy_coef", "temperature")
 
     @staticmethod
-    def _args(saved, key):
-        y, old, adv, ref, mask = saved
-        padidx, scalars = key
-        return (y.data_ptr(), padidx, _opt(mask), old.data_ptr(), adv.data_ptr(), adv.numel(), _opt(ref)) + scalars
-
-    @staticmethod
-    @_on_tensor_device
-    def forward(ctx, logits, targets, padidx, old_logp, advantages, ref_logp, clip_low, clip_high, kl_coef, entropy_coef,
-                temperature, mask, reduction, eager_grad):
+    def check(x, args):
         what = "policy_loss"
-        x, y, rows = _token_rows(what, logits, targets)
+        targets, padidx, old_logp, advantages, ref_logp, mask, *numbers = args
         lead = targets.shape
         old = _row_floats(what, "old_logp", old_logp, x, lead)
         _need(torch.is_tensor(advantages), f"{what}: advantages must be a floating tensor")
         per_column = len(lead) == 2 and advantages.shape == lead[1:]
         adv = _row_floats(what, "advantages", advantages, x, lead[1:] if per_column else lead)
         ref = None if ref_logp is None else _row_floats(what, "ref_logp", ref_logp, x, lead)
-        scalars = tuple(_float_arg(what, n, v) for n, v in (("clip_low", clip_low), ("clip_high", clip_high), ("kl_coef", kl_coef),
-                                                            ("entropy_coef", entropy_coef), ("temperature", temperature)))
-        _need(scalars[2] == 0.0 or ref is not None, f"{what}: kl_coef needs ref_logp")
-        ctx.key = (int(padidx), scalars)
-        saved = (y, old, adv, ref, _mask_bytes(what, mask, x, lead))
-        logp = torch.empty(lead, dtype=torch.float32, device=x.device)
-        entropy = torch.empty_like(logp)
-        loss = PolicyLossFn._run_forward(ctx, x, rows, logits.shape, lead, saved, reduction, eager_grad, (logp, entropy))
-        ctx.mark_non_differentiable(logp, entropy)
-        ctx.set_materialize_grads(False)
-        return loss, logp, entropy
+        numbers = tuple([_float_arg(what, n, v) for n, v in zip(_PolicyLoss.NUMBERS, numbers)])
+        _need(numbers[2] == 0.0 or ref is not None, f"{what}: kl_coef needs ref_logp")
+        return (old, adv, ref, _mask_bytes(what, mask, x, lead)), (int(padidx), numbers)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    @_on_tensor_device
-    def backward(ctx, g, _glogp, _gentropy):
-        return (PolicyLossFn._run_backward(ctx, g) if g is not None else None,) + (None,) * 13
+    def outputs(lead, dev):
+        logp = torch.empty(lead, dtype=torch.float32, device=dev)
+        return logp, torch.empty_like(logp)
+
+    @staticmethod
+    def pointers(saved, scalars):
+        old, adv, ref, mask = saved
+        padidx, numbers = scalars
+        return (padidx, None if mask is None else mask.data_ptr(), old.data_ptr(), adv.data_ptr(), adv.numel(),
+                None if ref is None else ref.data_ptr()) + numbers
 
 
 def policy_loss(logits, targets, padidx, old_logp, advantages, ref_logp=None, clip_low: float = 0.2, clip_high: float = 0.2,
@@ -998,8 +1030,10 @@ def policy_loss(logits, targets, padidx, old_logp, advantages, ref_logp=None, cl
     padidx or whose mask is false (a prompt's tokens) take no part.  Returns (loss, logp, entropy), the last two of
     targets' shape and without gradient; reduction and eager_grad as in distill_loss.  Differentiable in the logits
     alone."""
-    return PolicyLossFn.apply(logits, targets, padidx, old_logp, advantages, ref_logp, clip_low, clip_high, kl_coef, entropy_coef,
-                              temperature, mask, reduction, eager_grad)
+    args = (targets, padidx, old_logp, advantages, ref_logp, mask, clip_low, clip_high, kl_coef, entropy_coef, temperature)
+    if _grad_wanted(logits):
+        return RowLossFn.apply(logits, (_PolicyLoss, args, reduction, eager_grad))
+    return _row_loss_fwd(logits, _PolicyLoss, args, reduction, False)[0]
 
 
 class PreferenceLossFn(torch.autograd.Function):
@@ -1008,11 +1042,12 @@ class PreferenceLossFn(torch.autograd.Function):
 
     @staticmethod
     @_on_tensor_device
-    def forward(ctx, logits, targets, padidx, ref_logp, beta, label_smoothing, mask, batch_first, reduction):
+    def _forward(logits, targets, padidx, ref_logp, beta, label_smoothing, mask, batch_first, reduction):
         what = "preference_loss"
         x, y, rows = _token_rows(what, logits, targets)
         _need(targets.dim() == 2, f"{what}: targets must be (T, 2 P), or (2 P, T) with batch_first")
-        _need(reduction in _REDUCTIONS, f"{what}: reduction must be one of {sorted(_REDUCTIONS)}")
+        reduce_code = _REDUCTIONS.get(reduction)
+        _need(reduce_code is not None, f"{what}: reduction must be one of {sorted(_REDUCTIONS)}")
         S, T = targets.shape if batch_first else targets.shape[::-1]
         _need(S % 2 == 0, f"{what}: an even number of sequences is needed, the chosen ones first, then the rejected ones")
         ref = _row_floats(what, "ref_logp", ref_logp, x, (S,))
@@ -1020,39 +1055,45 @@ class PreferenceLossFn(torch.autograd.Function):
         beta, label_smoothing = _float_arg(what, "beta", beta), _float_arg(what, "label_smoothing", label_smoothing)
         L, dev, P = _lib.lib(), x.device, S // 2
         code, R, V, ld = rows
-        # for the backward: four numbers per row, one per sequence; here only: the call's workspace
+        # for the backward: four numbers per row and one per sequence; for this call alone: its workspace
         state = torch.empty((4 * R + S,), dtype=torch.float32, device=dev)
+        nbytes = L.gtg_preference_workspace_bytes(T, P)
+        ws = torch.empty((nbytes + 8,), dtype=torch.uint8, device=dev)
         seq_logp = torch.empty((S,), dtype=torch.float32, device=dev)
         pair_loss = torch.empty((P,), dtype=torch.float32, device=dev)
-        loss = torch.empty((), dtype=torch.float32, device=dev) if reduction != "none" else None
-        ws = _ws(L.gtg_preference_workspace_bytes(T, P), dev)
-        ctx.head = (code, T, P, V, ld, int(bool(batch_first)))
-        rc = L.gtg_preference_fwd(x.data_ptr(), *ctx.head, y.data_ptr(), int(padidx), _opt(m), ref.data_ptr(), beta, label_smoothing,
-                                  _REDUCTIONS[reduction], state.data_ptr(), state.data_ptr() + 16 * R, seq_logp.data_ptr(),
-                                  pair_loss.data_ptr(), _opt(loss), ws.data_ptr(), ws.numel(), stream_ptr())
+        loss = torch.empty((), dtype=torch.float32, device=dev) if reduce_code else None
+        head = (code, T, P, V, ld, int(bool(batch_first)))
+        rc = L.gtg_preference_fwd(x.data_ptr(), *head, y.data_ptr(), int(padidx), _opt(m), ref.data_ptr(), beta, label_smoothing,
+                                  reduce_code, state.data_ptr(), state.data_ptr() + 16 * R, seq_logp.data_ptr(),
+                                  pair_loss.data_ptr(), _opt(loss), ws.data_ptr(), nbytes, stream_ptr())
         if rc:
             check(rc, "gtg_preference_fwd")
-        ctx.save_for_backward(x, y, m, state)
-        ctx.padidx, ctx.scalar, ctx.shape, ctx.rows = int(padidx), loss is not None, logits.shape, rows
+        return pair_loss if loss is None else loss, seq_logp, (x, y, m, state), (head, int(padidx), loss is not None, logits.shape, rows)
+
+    @staticmethod
+    def forward(ctx, logits, args):
+        loss, seq_logp, saved, ctx.call = PreferenceLossFn._forward(logits, *args)
+        ctx.save_for_backward(*saved)
         ctx.mark_non_differentiable(seq_logp)
         ctx.set_materialize_grads(False)
-        return (pair_loss if loss is None else loss), seq_logp
+        return loss, seq_logp
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     @_on_tensor_device
     def backward(ctx, g, _gseq):
         if g is None:
-            return (None,) * 9
+            return None, None
         x, y, m, state = ctx.saved_tensors
+        head, padidx, scalar, shape, rows = ctx.call
         g = _f32c(g)
-        dx, ldg = _grad_like(x, ctx.shape, ctx.rows)
-        rc = _lib.lib().gtg_preference_bwd(x.data_ptr(), *ctx.head, y.data_ptr(), ctx.padidx, _opt(m), state.data_ptr(),
-                                           state.data_ptr() + 16 * ctx.rows[1], g.data_ptr() if ctx.scalar else None,
-                                           None if ctx.scalar else g.data_ptr(), dx.data_ptr(), ldg, stream_ptr())
+        dx, ldg = _grad_like(x, shape, rows)
+        rc = _lib.lib().gtg_preference_bwd(x.data_ptr(), *head, y.data_ptr(), padidx, _opt(m), state.data_ptr(),
+                                           state.data_ptr() + 16 * rows[1], g.data_ptr() if scalar else None,
+                                           None if scalar else g.data_ptr(), dx.data_ptr(), ldg, stream_ptr())
         if rc:
             check(rc, "gtg_preference_bwd")
-        return (dx,) + (None,) * 8
+        return dx, None
 
 
 def preference_loss(logits, targets, padidx, ref_logp, beta: float = 0.1, label_smoothing: float = 0.0, mask=None,
@@ -1067,4 +1108,5 @@ def preference_loss(logits, targets, padidx, ref_logp, beta: float = 0.1, label_
 
     Returns (loss, seq_logp (2 P), without gradient); reduction over the pairs: "mean", "sum" or "none".  Differentiable
     in the logits alone."""
-    return PreferenceLossFn.apply(logits, targets, padidx, ref_logp, beta, label_smoothing, mask, batch_first, reduction)
+    args = (targets, padidx, ref_logp, beta, label_smoothing, mask, batch_first, reduction)
+    return PreferenceLossFn.apply(logits, args) if _grad_wanted(logits) else PreferenceLossFn._forward(logits, *args)[:2]
