@@ -28,10 +28,32 @@ __device__ __forceinline__ float exp2_raw(float x) { return __builtin_amdgcn_exp
 // 16 bytes of logits, element by element as fp32.
 struct F32 {
     typedef float Store;
+    // the larger elements of the vectors taken, of every vector's first and second half (16-bit types: even and odd places)
+    struct Maxima {
+        float a = -__builtin_inff(), b = -__builtin_inff();
+        __device__ __forceinline__ void take(const u32x4& v)
+        {
+            a = fmaxf(fmaxf(a, get(v, 0)), get(v, 1));
+            b = fmaxf(fmaxf(b, get(v, 2)), get(v, 3));
+        }
+        __device__ __forceinline__ float lo() const { return a; }
+        __device__ __forceinline__ float hi() const { return b; }
+    };
     static constexpr int VEC = 4;
     static constexpr unsigned NEG2 = 0xff800000u;  // -inf in every element of a dword
     __device__ static float get(const u32x4& v, int q) { return __uint_as_float(v[q]); }
     __device__ static void clear(u32x4& v, int q) { v[q] = 0xff800000u; }
+    // element q, not known to the compiler, leaving -inf in its place
+    __device__ static float take(u32x4& v, int q)
+    {
+        unsigned d = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            d = q == i ? v[i] : d;
+            v[i] = q == i ? 0xff800000u : v[i];
+        }
+        return __uint_as_float(d);
+    }
     __device__ static float load(const Store* p) { return *p; }
     __device__ static Store cvt(float f) { return f; }
     __device__ static u32x4 pack(const float* f)
@@ -42,8 +64,29 @@ struct F32 {
         return v;
     }
 };
+// Without unpacking: 16-bit floats are in the order of their bits as integers where they are positive and in reverse where they are
+// negative, so the largest is the largest signed integer, or, if that is negative, the smallest unsigned one.
+template <unsigned NEG2, typename H>
+struct Maxima16 {
+    typedef short i16x2 __attribute__((ext_vector_type(2)));
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    unsigned p = NEG2, n = NEG2;
+    __device__ __forceinline__ void take(const u32x4& v)
+    {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const unsigned w = v[i];  // (a bit cast of v[i] itself would read v[0])
+            p = __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(i16x2, p), __builtin_bit_cast(i16x2, w)));
+            n = __builtin_bit_cast(unsigned, __builtin_elementwise_min(__builtin_bit_cast(u16x2, n), __builtin_bit_cast(u16x2, w)));
+        }
+    }
+    __device__ __forceinline__ float lo() const { return H::widen((p & 0x8000u) ? n & 0xffffu : p & 0xffffu); }
+    __device__ __forceinline__ float hi() const { return H::widen((p & 0x80000000u) ? n >> 16 : p >> 16); }
+};
 struct BF16 {
     typedef __bf16 Store;
+    __device__ static float widen(unsigned bits) { return __uint_as_float(bits << 16); }
+    typedef Maxima16<0xff80ff80u, BF16> Maxima;
     static constexpr int VEC = 8;
     static constexpr unsigned NEG2 = 0xff80ff80u;  // -inf in every element of a dword
     __device__ static float get(const u32x4& v, int q)
@@ -53,6 +96,19 @@ struct BF16 {
     __device__ static void clear(u32x4& v, int q)
     {
         v[q >> 1] = (q & 1) ? ((v[q >> 1] & 0xffffu) | 0xff800000u) : ((v[q >> 1] & 0xffff0000u) | 0xff80u);
+    }
+    __device__ static float take(u32x4& v, int q)
+    {
+        const int at = (q & 1) * 16;
+        unsigned d = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const bool here = q >> 1 == i;
+            d = here ? v[i] : d;
+            v[i] = here ? (v[i] & ~(0xffffu << at)) | (0xff80u << at) : v[i];
+        }
+        d = d >> at & 0xffffu;
+        return __uint_as_float(d << 16);
     }
     __device__ static float load(const Store* p) { return (float)*p; }
     __device__ static Store cvt(float f) { return (__bf16)f; }
@@ -69,6 +125,8 @@ struct BF16 {
 };
 struct F16 {
     typedef _Float16 Store;
+    __device__ static float widen(unsigned bits) { return (float)__builtin_bit_cast(_Float16, (unsigned short)bits); }
+    typedef Maxima16<0xfc00fc00u, F16> Maxima;
     static constexpr int VEC = 8;
     static constexpr unsigned NEG2 = 0xfc00fc00u;  // -inf in every element of a dword
     __device__ static float get(const u32x4& v, int q)
@@ -78,6 +136,19 @@ struct F16 {
     __device__ static void clear(u32x4& v, int q)
     {
         v[q >> 1] = (q & 1) ? ((v[q >> 1] & 0xffffu) | 0xfc000000u) : ((v[q >> 1] & 0xffff0000u) | 0xfc00u);
+    }
+    __device__ static float take(u32x4& v, int q)
+    {
+        const int at = (q & 1) * 16;
+        unsigned d = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const bool here = q >> 1 == i;
+            d = here ? v[i] : d;
+            v[i] = here ? (v[i] & ~(0xffffu << at)) | (0xfc00u << at) : v[i];
+        }
+        d = d >> at & 0xffffu;
+        return (float)__builtin_bit_cast(_Float16, (unsigned short)d);
     }
     __device__ static float load(const Store* p) { return (float)*p; }
     __device__ static Store cvt(float f) { return (_Float16)f; }
@@ -987,12 +1058,12 @@ __device__ __forceinline__ unsigned order_key(float x)
     return x != x ? 0xffffffffu : (b & 0x80000000u) ? ~b : b | 0x80000000u;
 }
 
-// The usual way takes two sweeps.  The first finds maxima of parts of the row, one per thread (two, over the vectors' halves,
+// The usual way takes two sweeps.  The first finds maxima of parts of the row, one per thread (two, of halves of its vectors,
 // for a k that is not small beside the threads): the k-th largest of them is a bound that at least k elements reach and few
 // more do.  The second puts what reaches the bound on a list and sums the exponentials of everything below, relative to
 // the bound.  The list's elements then find their rank by comparing with each other.  Where the list would overflow (many equal
-// values), or a NaN is about, the k-th largest is found bit by bit with a sweep for each; where what lies below the bound vanishes
-// beside it, the tail is summed in two more sweeps relative to its own maximum.
+// values), or a NaN is about, the k-th largest is found bit by bit with a sweep for each; where what lies below the bound
+// vanishes beside it, the tail is summed in two more sweeps relative to its own maximum.
 constexpr int TOP_LIST = 1024;
 
 __device__ __forceinline__ float key_value(unsigned key)  // the float of a key that is no NaN's
@@ -1031,13 +1102,16 @@ __device__ __forceinline__ unsigned kth_key16(const unsigned* keys, int n, int k
 }
 
 template <typename E, int NT, int NV>
-__global__ __launch_bounds__(NT, min_waves(NV)) void top_kernel(const void* logits, int64_t ld, int64_t first, int V, int k,
+__global__ __launch_bounds__(NT, NV == 8 ? 8 : min_waves(NV)) void top_kernel(const void* logits, int64_t ld, int64_t first, int V, int k,
                                                                 double inv_tau, void* __restrict__ values,
                                                                 int32_t* __restrict__ indices, float* __restrict__ tail)
 {
     __shared__ float shf[16];
     __shared__ int sh[16];
+    constexpr int NW = NT / 64, ASIDE = NT == 1024 ? 64 : NT == 512 ? 96 : NT == 256 ? 160 : 256;  // vectors put aside per wave
     __shared__ int fill;
+    __shared__ u32x4 aside_vec[NW * ASIDE];
+    __shared__ int aside_j[NW * ASIDE];
     __shared__ unsigned bound_key, kth_key;
     __shared__ int kth_idx;
     __shared__ unsigned long long list[TOP_LIST];  // key, then the complement of the index: larger is nearer the front
@@ -1051,15 +1125,9 @@ __global__ __launch_bounds__(NT, min_waves(NV)) void top_kernel(const void* logi
     const float c = (float)(LOG2E * inv_tau);
 
     const bool halves = 4 * k > NT;
-    float lo = neg_inf(), hi = neg_inf();
-    row.template each<true>([&](int, const u32x4& v) {
-#pragma unroll
-        for (int q = 0; q < E::VEC / 2; ++q) {
-            lo = fmaxf(lo, E::get(v, q));
-            hi = fmaxf(hi, E::get(v, q + E::VEC / 2));
-        }
-    });
-    lo = fmaxf(lo, row.xe);
+    typename E::Maxima parts;
+    row.template each<true>([&](int, const u32x4& v) { parts.take(v); });
+    const float lo = fmaxf(parts.lo(), row.xe), hi = parts.hi();
     keys[tid] = order_key(halves ? lo : fmaxf(lo, hi));
     if (halves) keys[NT + tid] = order_key(hi);
     if (tid == 0) fill = 0;
@@ -1076,31 +1144,52 @@ __global__ __launch_bounds__(NT, min_waves(NV)) void top_kernel(const void* logi
     };
     const Scale sc(bound, c);
     float s = 0.f;
+    const int wave = tid >> 6, lane = tid & 63;
+    u32x4* vec_aside = &aside_vec[wave * ASIDE];
+    int* j_aside = &aside_j[wave * ASIDE];
+    int na = 0;  // the same in every lane
     row.template each<false>([&](int j, u32x4& v) {
-        const float vm = vec_max<E>(neg_inf(), v);
-        if (!(vm < bound)) {
-            int n = 0;
-#pragma unroll
-            for (int q = 0; q < E::VEC; ++q) n += !(E::get(v, q) < bound) ? 1 : 0;
-            int at = atomicAdd(&fill, n);
-#pragma unroll
-            for (int q = 0; q < E::VEC; ++q) {
-                const float f = E::get(v, q);
-                if (!(f < bound)) {
-                    put(at++, j + q, f);
-                    E::clear(v, q);
+        const bool hit = !(vec_max<E>(neg_inf(), v) < bound);
+        const unsigned long long hits = __ballot(hit);
+        if (hits) {
+            // (two of three wave-wide vectors hold one of 64 elements out of 30 522: here they are only put aside)
+            const int at = na + (int)__builtin_amdgcn_mbcnt_hi((unsigned)(hits >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)hits, 0));
+            if (hit) {
+                if (at < ASIDE) {
+                    vec_aside[at] = v;
+                    j_aside[at] = j;
                 }
+                v = u32x4{E::NEG2, E::NEG2, E::NEG2, E::NEG2};
             }
+            na += __popcll(hits);
         }
 #pragma unroll
-        for (int q = 0; q < E::VEC; ++q) s += exp2_raw(sc.y(E::get(v, q)));  // (a NaN that vm passed over shows in the sum)
+        for (int q = 0; q < E::VEC; ++q) s += exp2_raw(sc.y(E::get(v, q)));  // (a NaN that the maximum passed over shows in the sum)
     });
     if (row.je >= 0) {
         if (row.xe < bound) s += exp2_raw(sc.y(row.xe));
         else put(atomicAdd(&fill, 1), row.je, row.xe);
     }
+    // (lanes past the row's end have missed the last vectors' count; the largest is the wave's)
+    na = wave_reduce(na, [](int a, int b) { return max(a, b); });
+    if (na > ASIDE && lane == 0) atomicAdd(&fill, TOP_LIST + 1);
+    for (int i = lane; i < min(na, ASIDE); i += 64) {
+        u32x4 v = vec_aside[i];
+        const int j = j_aside[i];
+        unsigned found = 0;
+#pragma unroll
+        for (int q = 0; q < E::VEC; ++q) found |= !(E::get(v, q) < bound) ? 1u << q : 0u;
+        int at = atomicAdd(&fill, __popc(found));
+        while (found) {
+            const int q = __ffs(found) - 1;
+            found &= found - 1;
+            put(at++, j + q, E::take(v, q));
+        }
+#pragma unroll
+        for (int q = 0; q < E::VEC; ++q) s += exp2_raw(sc.y(E::get(v, q)));
+    }
     s = block_sum<NT, false>(s, shf);
-    if (NT == 64) __syncthreads();
+    __syncthreads();
     int n = fill;
     const bool exact = n > TOP_LIST || s != s;
     Row<E, NT, 0> again(x, V);  // the rare ways read the row anew: their loops need no registers of the usual one's
@@ -1142,8 +1231,7 @@ __global__ __launch_bounds__(NT, min_waves(NV)) void top_kernel(const void* logi
     }
     // ranks: a wave compares 64 of the list's elements with its share of the whole list
     {
-        constexpr int NW = NT / 64;
-        const int w = tid >> 6, lane = tid & 63;
+        const int w = wave;
         const int share = (n + NW - 1) / NW, o0 = w * share, o1 = min(n, o0 + share);
         for (int i0 = 0; i0 < n; i0 += 64) {
             const unsigned long long mine = list[min(i0 + lane, n - 1)];
@@ -1296,6 +1384,13 @@ void by_vectors(int64_t n, F launch)
     else if (n <= 16384) launch(Shape<E, 1024, 16>());
     else launch(Shape<E, 512, 0>());
 }
+// For the k largest at least 256 threads beyond the smallest rows: as many maxima bound the k-th.
+template <typename E, typename F>
+void by_vectors_top(int64_t n, F launch)
+{
+    if (n > 64 && n <= 256) launch(Shape<E, 256, 4>());
+    else by_vectors<E>(n, launch);
+}
 template <typename F>
 void by_size(int dtype, int vocab, F launch)
 {
@@ -1324,13 +1419,17 @@ int top_logits(const void* logits, int dtype, int64_t R, int V, int64_t ld, int 
 {
     ProfScope prof(s, "top_logits", R, V, k);
     const double it = 1.0 / temperature;
-    by_size(dtype, V, [&](auto shape) {
+    auto launch = [&](auto shape) {
         typedef decltype(shape) P;
         by_slices(R, [&](int64_t r0, unsigned n) {
             hipLaunchKernelGGL(HIP_KERNEL_NAME(top_kernel<typename P::E, P::NT, P::NV>), dim3(n), dim3(P::NT), 0, s, logits, ld, r0,
                                V, k, it, values, indices, tail);
         });
-    });
+    };
+    const int64_t vectors = ((int64_t)V * (dtype == GTG_DTYPE_F32 ? 4 : 2) + 15) / 16;
+    if (dtype == GTG_DTYPE_F32) by_vectors_top<F32>(vectors, launch);
+    else if (dtype == GTG_DTYPE_F16) by_vectors_top<F16>(vectors, launch);
+    else by_vectors_top<BF16>(vectors, launch);
     return check_launch("top_kernel");
 }
 
