@@ -172,6 +172,29 @@ class DAE(TextModel):
         mask = targets != self.padidx
         return (((pred == targets) & mask).sum() / mask.sum()).item()
 
+    # Beyond teacher forcing (no counterpart in the reference): what a trained decoder is distilled, scored and tuned
+    # with, on the logits (T, B, vocab) that ``decode`` returns and tokens (T, B); pad tokens take no part.  On the GPU only.
+    def top_logits(self, logits, k, temperature=1.0):
+        """A teacher's answer in short: (values, indices (T, B, k), tail (T, B)); see functional.top_logits."""
+        return Fn.top_logits(logits, k, temperature)
+
+    def token_logprob(self, logits, targets, temperature=1.0):
+        """(log-probability of the targets, entropy) per token; see functional.token_logprob."""
+        return Fn.token_logprob(logits, targets, self.padidx, temperature)
+
+    def loss_distill(self, logits, targets, values, indices, tail=None, temperature=1.0, ce_weight=0.0, **kw):
+        """Loss against what a teacher's ``top_logits`` returned; see functional.distill_loss."""
+        return Fn.distill_loss(logits, values, indices, targets, self.padidx, tail, temperature, ce_weight, **kw)
+
+    def loss_policy(self, logits, targets, old_logp, advantages, ref_logp=None, **kw):
+        """Clipped policy loss of sampled tokens: (loss, logp, entropy); see functional.policy_loss."""
+        return Fn.policy_loss(logits, targets, self.padidx, old_logp, advantages, ref_logp, **kw)
+
+    def loss_preference(self, logits, targets, ref_logp, **kw):
+        """Loss of the first half of the batch's sentences, preferred over the second half: (loss, each sentence's
+        log-probability); see functional.preference_loss."""
+        return Fn.preference_loss(logits, targets, self.padidx, ref_logp, **kw)
+
     def autoenc(self, inputs, targets):
         return self(inputs)
 
