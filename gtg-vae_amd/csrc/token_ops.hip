@@ -1059,31 +1059,27 @@ __device__ __forceinline__ unsigned order_key(float x)
 }
 
 // The usual way takes two sweeps.  The first finds maxima of parts of the row, one per thread (two, of halves of its vectors,
-// for a k that is not small beside the threads): the k-th largest of them is a bound that at least k elements reach and few
-// more do.  The second puts what reaches the bound on a list and sums the exponentials of everything below, relative to
-// the bound.  The list's elements then find their rank by comparing with each other.  Where the list would overflow (many equal
+// for a k that is not small beside the threads; up to eight where one wave has the row): the k-th largest of them is a bound
+// that at least k elements reach and few more do.  The second puts what reaches the bound on a list and sums the exponentials
+// of everything below, relative to the bound.  The list's elements then find their rank by comparing with each other.  Where the list would overflow (many equal
 // values), or a NaN is about, the k-th largest is found bit by bit with a sweep for each; where what lies below the bound
 // vanishes beside it, the tail is summed in two more sweeps relative to its own maximum.
-constexpr int TOP_LIST = 1024;
 
 __device__ __forceinline__ float key_value(unsigned key)  // the float of a key that is no NaN's
 {
     return __uint_as_float((key & 0x80000000u) ? key ^ 0x80000000u : ~key);
 }
 
-// One wave: the k-th largest of the n keys (a multiple of 64, at most 64 N), to 16 bits and rounded down.  The bits above the
-// highest one in which any two keys differ are common to all.
+// One wave: the k-th largest of its 64 N keys, to 16 bits and rounded down.  The bits above the highest one in which any two
+// keys differ are common to all.
 template <int N>
-__device__ __forceinline__ unsigned kth_key16(const unsigned* keys, int n, int k)
+__device__ __forceinline__ unsigned kth_key16(const unsigned (&mk)[N], int k)
 {
-    unsigned mk[N], all_or = 0, all_and = 0xffffffffu;
+    unsigned all_or = 0, all_and = 0xffffffffu;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        mk[i] = 64 * i < n ? keys[(threadIdx.x & 63) + 64 * i] : 0;
-        if (64 * i < n) {
-            all_or |= mk[i];
-            all_and &= mk[i];
-        }
+        all_or |= mk[i];
+        all_and &= mk[i];
     }
     const unsigned differ = (unsigned)wave_reduce((int)all_or, [](int a, int b) { return a | b; }) ^
                             (unsigned)wave_reduce((int)all_and, [](int a, int b) { return a & b; });
@@ -1094,21 +1090,33 @@ __device__ __forceinline__ unsigned kth_key16(const unsigned* keys, int n, int k
         const unsigned cand = kth | (1u << bit);
         int c = 0;
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (64 * i < n) c += __popcll(__ballot(mk[i] >= cand));
+        for (int i = 0; i < N; ++i) c += __popcll(__ballot(mk[i] >= cand));
         if (c >= k) kth = cand;
     }
     return kth & 0xffff0000u;
 }
+template <int N>
+__device__ __forceinline__ unsigned kth_key16_of(const unsigned* keys, int k)
+{
+    unsigned mk[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) mk[i] = keys[(threadIdx.x & 63) + 64 * i];
+    return kth_key16<N>(mk, k);
+}
 
 template <typename E, int NT, int NV>
-__global__ __launch_bounds__(NT, NV == 8 ? 8 : min_waves(NV)) void top_kernel(const void* logits, int64_t ld, int64_t first, int V, int k,
+__global__ __launch_bounds__(NT, NT == 64 ? 3 : NT == 256 ? 6 : NV == 8 ? 8 : min_waves(NV)) void top_kernel(const void* logits, int64_t ld, int64_t first, int V, int k,
                                                                 double inv_tau, void* __restrict__ values,
                                                                 int32_t* __restrict__ indices, float* __restrict__ tail)
 {
     __shared__ float shf[16];
     __shared__ int sh[16];
-    constexpr int NW = NT / 64, ASIDE = NT == 1024 ? 64 : NT == 512 ? 96 : NT == 256 ? 160 : 256;  // vectors put aside per wave
+    // places for listed elements, and per wave for vectors put aside
+    // (k = 256 lists about 350 elements, which one wave finds in 250 vectors out of 512 and in 300 out of 1024)
+    constexpr int NW = NT / 64, TOP_LIST = NT == 64 ? 512 : 1024;
+    constexpr int ASIDE = NT == 1024 ? 64 : NT == 512 ? 96 : NT == 256 ? 160 : NV == 16 ? 384 : NV == 8 ? 320 : NV == 4 ? 256 : 64;
+    static_assert(NT > 64 || NV > 0, "a streamed row has more than one wave");
+    constexpr int SPARE = NT == 64 ? TOP_LIST : 2 * NT;
     __shared__ int fill;
     __shared__ u32x4 aside_vec[NW * ASIDE];
     __shared__ int aside_j[NW * ASIDE];
@@ -1116,7 +1124,7 @@ __global__ __launch_bounds__(NT, NV == 8 ? 8 : min_waves(NV)) void top_kernel(co
     __shared__ int kth_idx;
     __shared__ unsigned long long list[TOP_LIST];  // key, then the complement of the index: larger is nearer the front
     __shared__ int ranks[TOP_LIST];
-    __shared__ unsigned keys[2 * NT];              // maxima; then the floats that are listed but not among the k, in order
+    __shared__ unsigned keys[SPARE];               // maxima; then the floats that are listed but not among the k, in order
     const int64_t r = first + blockIdx.x;
     const int tid = threadIdx.x;
     const typename E::Store* x = reinterpret_cast<const typename E::Store*>(logits) + r * ld;
@@ -1124,18 +1132,37 @@ __global__ __launch_bounds__(NT, NV == 8 ? 8 : min_waves(NV)) void top_kernel(co
     row.load();
     const float c = (float)(LOG2E * inv_tau);
 
-    const bool halves = 4 * k > NT;
-    typename E::Maxima parts;
-    row.template each<true>([&](int, const u32x4& v) { parts.take(v); });
-    const float lo = fmaxf(parts.lo(), row.xe), hi = parts.hi();
-    keys[tid] = order_key(halves ? lo : fmaxf(lo, hi));
-    if (halves) keys[NT + tid] = order_key(hi);
     if (tid == 0) fill = 0;
     for (int i = tid; i < TOP_LIST; i += NT) ranks[i] = 0;
-    __syncthreads();
-    if (tid < 64) {
-        const unsigned key = halves ? kth_key16<2 * NT / 64>(keys, 2 * NT, k) : kth_key16<NT / 64>(keys, NT, k);
+    if constexpr (NT == 64) {
+        // one wave: up to eight maxima a lane, of the halves of every vector or every few, and no LDS
+        constexpr int PARTS = NV < 4 ? NV : 4, EACH = NV / PARTS;
+        unsigned mk[2 * PARTS];
+        float single = row.xe;
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i) {
+            typename E::Maxima part;
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) part.take(row.v[i * EACH + e]);
+            mk[2 * i] = order_key(fmaxf(part.lo(), single));
+            mk[2 * i + 1] = order_key(part.hi());
+            single = neg_inf();
+        }
+        // (a row of so few vectors that it has fewer maxima than k is listed whole)
+        const unsigned key = k > 128 * PARTS ? 0u : kth_key16<2 * PARTS>(mk, k);
         if (tid == 0) bound_key = key;
+    } else {
+        const bool halves = 4 * k > NT;
+        typename E::Maxima parts;
+        row.template each<true>([&](int, const u32x4& v) { parts.take(v); });
+        const float lo = fmaxf(parts.lo(), row.xe), hi = parts.hi();
+        keys[tid] = order_key(halves ? lo : fmaxf(lo, hi));
+        if (halves) keys[NT + tid] = order_key(hi);
+        __syncthreads();
+        if (tid < 64) {
+            const unsigned key = halves ? kth_key16_of<2 * NT / 64>(keys, k) : kth_key16_of<NT / 64>(keys, k);
+            if (tid == 0) bound_key = key;
+        }
     }
     __syncthreads();
     const float bound = bound_key > order_key(neg_inf()) ? key_value(bound_key) : neg_inf();
@@ -1243,7 +1270,7 @@ __global__ __launch_bounds__(NT, NV == 8 ? 8 : min_waves(NV)) void top_kernel(co
     }
     __syncthreads();
     float* rest = reinterpret_cast<float*>(keys);
-    const bool spare = n - k <= 2 * NT;  // (the maxima's places hold what is listed beyond k; more than they are goes the long way)
+    const bool spare = n - k <= SPARE;  // (the maxima's places hold what is listed beyond k; more than they are goes the long way)
     for (int i = tid; i < n; i += NT) {
         const unsigned key = (unsigned)(list[i] >> 32);
         const int j = (int)~(unsigned)list[i], rank = ranks[i];
@@ -1366,37 +1393,36 @@ __global__ __launch_bounds__(1024) void prefer_kernel(Prefer a)
 }
 
 // A block per row, by the row's 16-byte vectors: as many threads as they keep busy, and the row in registers up to 16 vectors
-// (64 registers) a thread and 1024 threads -- 128 K elements of 16 bits, 64 K of 32.
+// (64 registers) a thread and 1024 threads -- 128 K elements of 16 bits, 64 K of 32.  One wave for up to 512 vectors: a block
+// of four has a quarter of the lanes idle there and passes sums through LDS (40 000 rows of 2500 bf16: log-probability 82 us with
+// 256 threads, 45 with 64; policy loss 154 and 92; the k largest 200 and 140).  From 513 to 1024 two waves, but one for the
+// k largest, which has no LDS to wait for then: 40 000 rows of 2500 fp32 169 and 142 us; the distillation 187 with two, 198 with one.
+// One wave is slow to rank a long list, though: above k = 64 the rows of 257 to 1024 vectors take four (k = 256, 20 000 rows of
+// 4000 fp32: 635 us with one, 406 with four; k = 64 141 and 130, and of 2000 fp32 207 and 238).
 template <typename E_, int NT_, int NV_>
 struct Shape {
     typedef E_ E;
     static constexpr int NT = NT_, NV = NV_;
 };
-template <typename E, typename F>
+template <typename E, int MID, typename F>
 void by_vectors(int64_t n, F launch)
 {
     if (n <= 64) launch(Shape<E, 64, 1>());
     else if (n <= 256) launch(Shape<E, 64, 4>());
-    else if (n <= 1024) launch(Shape<E, 256, 4>());
+    else if (MID < 256 && n <= 512) launch(Shape<E, 64, MID < 256 ? 8 : 4>());
+    else if (n <= 1024) launch(Shape<E, MID, 1024 / MID>());
     else if (n <= 2048) launch(Shape<E, 256, 8>());
     else if (n <= 4096) launch(Shape<E, 512, 8>());
     else if (n <= 8192) launch(Shape<E, 512, 16>());
     else if (n <= 16384) launch(Shape<E, 1024, 16>());
     else launch(Shape<E, 512, 0>());
 }
-// For the k largest at least 256 threads beyond the smallest rows: as many maxima bound the k-th.
-template <typename E, typename F>
-void by_vectors_top(int64_t n, F launch)
-{
-    if (n > 64 && n <= 256) launch(Shape<E, 256, 4>());
-    else by_vectors<E>(n, launch);
-}
-template <typename F>
+template <int MID = 128, typename F>
 void by_size(int dtype, int vocab, F launch)
 {
-    if (dtype == GTG_DTYPE_F32) by_vectors<F32>(((int64_t)vocab + 3) / 4, launch);
-    else if (dtype == GTG_DTYPE_F16) by_vectors<F16>(((int64_t)vocab + 7) / 8, launch);
-    else by_vectors<BF16>(((int64_t)vocab + 7) / 8, launch);
+    if (dtype == GTG_DTYPE_F32) by_vectors<F32, MID>(((int64_t)vocab + 3) / 4, launch);
+    else if (dtype == GTG_DTYPE_F16) by_vectors<F16, MID>(((int64_t)vocab + 7) / 8, launch);
+    else by_vectors<BF16, MID>(((int64_t)vocab + 7) / 8, launch);
 }
 
 Rows as_rows(const TokenRows& t, int64_t first = 0, unsigned n = 0)
@@ -1426,10 +1452,8 @@ int top_logits(const void* logits, int dtype, int64_t R, int V, int64_t ld, int 
                                V, k, it, values, indices, tail);
         });
     };
-    const int64_t vectors = ((int64_t)V * (dtype == GTG_DTYPE_F32 ? 4 : 2) + 15) / 16;
-    if (dtype == GTG_DTYPE_F32) by_vectors_top<F32>(vectors, launch);
-    else if (dtype == GTG_DTYPE_F16) by_vectors_top<F16>(vectors, launch);
-    else by_vectors_top<BF16>(vectors, launch);
+    if (k > 64) by_size<256>(dtype, V, launch);
+    else by_size<64>(dtype, V, launch);
     return check_launch("top_kernel");
 }
 

@@ -126,6 +126,21 @@ def test_top_logits_ties_zeros_masks_and_nan(V, dtype):
         _check_top(x, k)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [200, 256, 257, 300, 511, 512, 1024, 2048, 4096, 8192])
+def test_top_logits_of_many_out_of_few(V, dtype):
+    """A k near the vocabulary's size, or beyond the number of parts whose maxima bound it, where the maxima are alike and the
+    rest far below; and rows whose largest lie next to each other."""
+    g = torch.Generator().manual_seed(V)
+    low = torch.rand(V, generator=g) - 40
+    low[::4] = 1 + torch.rand((V + 3) // 4, generator=g)
+    run = torch.randn(V, generator=g)
+    run[V // 3: V // 3 + 150] += 20
+    x = torch.stack([low, low.flip(0), run, torch.randn(V, generator=g).sort()[0]]).to(dtype)
+    for k in (min(V, 256), 199, 129, 128):
+        _check_top(x, k)
+
+
 def test_top_logits_takes_strides_and_other_shapes():
     Fn = _fn()
     x, _, _ = _logits(6, 5, 1003, torch.bfloat16, seed=1)
