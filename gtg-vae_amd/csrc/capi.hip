@@ -1448,12 +1448,15 @@ static bool aligned_to(const void* p, size_t a) { return reinterpret_cast<uintpt
         GTG_REQUIRE((rows) == 0 || (dlogits) != (logits), "dlogits must not overlap the logits");                         \
     } while (0)
 
+// (beyond these the fp32 factors log2(e) / temperature and its products with gradients leave their range)
+static bool good_temperature(double t) { return t >= 1e-6 && t <= 1e6; }
+
 int gtg_top_logits(const void* logits, int dtype, int64_t rows, int vocab, int64_t ld, int k, double temperature,
                    void* values, int32_t* indices, float* tail, void* stream)
 {
     GTG_REQUIRE_LOGITS(logits, dtype, rows, vocab, ld);
     GTG_REQUIRE(k >= 1 && k <= 256 && k <= vocab, "k must be in [1, min(vocab, 256)]");
-    GTG_REQUIRE(temperature > 0 && std::isfinite(temperature), "temperature must be positive");
+    GTG_REQUIRE(good_temperature(temperature), "temperature must be in [1e-6, 1e6]");
     if (rows == 0) return GTG_OK;
     GTG_REQUIRE(values && indices && tail, "null pointer");
     GTG_REQUIRE(aligned_to(values, dtype_size(dtype)), "values: misaligned");
@@ -1464,7 +1467,7 @@ int gtg_token_logprob_fwd(const void* logits, int dtype, int64_t rows, int vocab
                           int64_t padidx, double temperature, float* logp, float* entropy, float* stats, void* stream)
 {
     GTG_REQUIRE_LOGITS(logits, dtype, rows, vocab, ld);
-    GTG_REQUIRE(temperature > 0 && std::isfinite(temperature), "temperature must be positive");
+    GTG_REQUIRE(good_temperature(temperature), "temperature must be in [1e-6, 1e6]");
     if (rows == 0) return GTG_OK;
     GTG_REQUIRE(targets && logp && entropy, "null pointer");
     GTG_REQUIRE(stats == nullptr || aligned_to(stats, 16), "stats: misaligned");
@@ -1478,7 +1481,7 @@ int gtg_token_logprob_bwd(const void* logits, int dtype, int64_t rows, int vocab
 {
     GTG_REQUIRE_LOGITS(logits, dtype, rows, vocab, ld);
     GTG_REQUIRE_GRADIENT(logits, dtype, rows, vocab, dlogits, ldg);
-    GTG_REQUIRE(temperature > 0 && std::isfinite(temperature), "temperature must be positive");
+    GTG_REQUIRE(good_temperature(temperature), "temperature must be in [1e-6, 1e6]");
     if (rows == 0) return GTG_OK;
     GTG_REQUIRE(targets && stats && aligned_to(stats, 16), "null or misaligned pointer");
     const TokenRows t{logits, dtype, rows, vocab, ld, targets, padidx, nullptr};
@@ -1491,7 +1494,7 @@ static const char* distill_fault(int vocab, const void* values, int value_dtype,
     if (dtype_size(value_dtype) == 0) return "value_dtype must be GTG_DTYPE_F32, _F16 or _BF16";
     if (k < 1 || k > 256) return "k must be in [1, 256]";
     if (vocab > distill_max_vocab()) return "vocab must be at most 400 000";
-    if (!(temperature > 0) || !std::isfinite(temperature)) return "temperature must be positive";
+    if (!good_temperature(temperature)) return "temperature must be in [1e-6, 1e6]";
     if (!(ce_weight >= 0 && ce_weight <= 1)) return "ce_weight must be in [0, 1]";
     if (rows > 0 && (!values || !indices || !aligned_to(values, dtype_size(value_dtype)))) return "null or misaligned pointer";
     return nullptr;
@@ -1541,7 +1544,7 @@ int gtg_distill_loss_bwd(const void* logits, int dtype, int64_t rows, int vocab,
 
 static const char* policy_fault(const PolicyRows& p, const int64_t* targets, int64_t rows)
 {
-    if (!(p.temperature > 0) || !std::isfinite(p.temperature)) return "temperature must be positive";
+    if (!good_temperature(p.temperature)) return "temperature must be in [1e-6, 1e6]";
     if (!(p.clip_low >= 0) || !(p.clip_high >= 0)) return "clip_low and clip_high must not be negative";
     if (!std::isfinite(p.kl_coef) || !std::isfinite(p.entropy_coef)) return "kl_coef and entropy_coef must be finite";
     if (rows > 0 && p.adv_rows < 1) return "adv_rows must be positive";

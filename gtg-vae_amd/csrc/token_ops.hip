@@ -437,8 +437,9 @@ __device__ __forceinline__ double log_row(double x)
     return x == 0.0 ? -__builtin_inf() : x == __builtin_inf() ? x : l;
 }
 __device__ __forceinline__ float finite_or_zero(float m) { return m == neg_inf() ? 0.f : m; }
-// x - m, from below at the lowest finite number: its product with exp(-inf) = 0 is then 0 and not NaN
-__device__ __forceinline__ float clamped(float d) { return fmaxf(d, -3.402823466e38f); }
+// An exponent from below at -1024, where its power is 0 already: what is multiplied with that 0 -- the exponent itself, or its
+// product with a gradient's coefficient -- then stays finite and the product is 0, not NaN (masked logits).
+__device__ __forceinline__ float clamped(float d) { return fmaxf(d, -1024.f); }
 
 // ---- which rows count -------------------------------------------------------------------------------------------
 struct Rows {

@@ -422,7 +422,7 @@ int gtg_dropout(const float* x, int64_t count, float p, uint64_t seed, uint64_t 
  *   targets (rows) int64: the row's token.  A row whose target equals padidx, or whose mask byte (rows, uint8,
  *     nullable) is 0, is not read; its outputs, its loss and its gradient are zero.  A target outside [0, vocab) that
  *     is not padidx gives NaN in the row's outputs and gradient.
- *   temperature > 0: everything is a function of logits / temperature.
+ *   temperature in [1e-6, 1e6]: everything is a function of logits / temperature.
  *   dlogits: the gradient, of the logits' type, row r at dlogits + r ldg, all `vocab` elements of every row written
  *     (zeros where the row does not count); must not overlap the logits.  Stored fastest where a row's address modulo 16 is
  *     that of its logits.

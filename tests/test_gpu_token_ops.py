@@ -218,6 +218,43 @@ def test_masked_logits_and_rows_that_do_not_count(dtype):
     _check_grad(got, want, torch.ones(T, B, 1), _delta(x)[0])
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [40, 1201, 9001, 140003])
+def test_masked_logits_under_large_entropy_gradients(V, dtype):
+    """Masked places, -inf or the type's lowest value, take no gradient however large what comes from above: a temperature
+    below 1, the scale of a gradient scaler, a sum over rows."""
+    T, B, tau, up = 2, 3, 0.5, 512.0
+    x, y, _ = _logits(T, B, V, dtype, seed=V, spread=4.0)
+    x[0, :, V // 3: V // 2] = -math.inf
+    x[1, :, V // 3: V // 2] = torch.finfo(dtype).min
+    x[1, 2, 1:] = -math.inf                # one class left
+    y = y % (V // 3)
+    delta, D = _delta(x, tau)
+    logp = torch.log_softmax(x.double() / tau, -1)
+    p = logp.exp()
+    logp = torch.where(p > 0, logp, 0.0)
+    want = -up / tau * p * (logp - (p * logp).sum(-1, keepdim=True))       # of up times the entropy
+    scale = torch.full((T, B, 1), up * (D + 12) / tau)
+    xg, yc, none = x.cuda().requires_grad_(True), y.cuda(), torch.zeros(T, B, device="cuda")
+    (got,) = torch.autograd.grad(up * _fn().token_logprob(xg, yc, -1, tau)[1].sum(), (xg,))
+    _check_grad(got, want, scale, delta, "entropy")
+    for eager in (True, False):
+        loss = _fn().policy_loss(xg, yc, -1, none, none, entropy_coef=0.25, temperature=tau, reduction="sum", eager_grad=eager)[0]
+        (got,) = torch.autograd.grad(-4 * up * loss, (xg,))
+        _check_grad(got, want, scale, delta, "policy")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_preference_with_masked_logits(dtype):
+    T, P, V = 4, 2, 700
+    x, y, g = _logits(T, 2 * P, V, dtype, seed=21)
+    x[0, :, 300:] = -math.inf
+    x[1, :, 300:] = torch.finfo(dtype).min
+    y = y % 300
+    seq = O.token_logprob(x.double(), y, 0)[0].sum(0)
+    _check_prefer(x, y, (seq + torch.randn((2 * P,), generator=g)).float())
+
+
 def test_rows_of_minus_infinity_bad_targets_and_nan_are_loud():
     x = torch.randn(5, 300).cuda()
     x[0] = -math.inf

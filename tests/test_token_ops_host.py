@@ -151,3 +151,10 @@ def test_python_functions_refuse_cpu_tensors():
                  lambda: Fn.policy_loss(x, y, 0, f, f), lambda: Fn.preference_loss(x, y, 0, f[0])):
         with pytest.raises(_lib.GtgError):
             call()
+
+
+def test_temperatures_out_of_range_are_refused():
+    for t in (1e-7, 1e7, 1e-300, 1e300):
+        refused("gtg_top_logits", *OK, 3, t, P, P, P, None, part="temperature")
+        refused("gtg_token_logprob_fwd", *OK, P, 0, t, P, P, P, None, part="temperature")
+        refused("gtg_token_logprob_bwd", *OK, P, 0, t, P, P, P, Q, 50, None, part="temperature")
