@@ -2,7 +2,8 @@
 
 PyTorch is used for device memory, streams and the autograd graph only; every
 arithmetic step of forward and backward runs in csrc/*.hip.  All tensors must
-be fp32 and on the GPU; there is no fallback.
+be on the GPU, and fp32 but for the operators on rows of vocabulary logits, which
+take fp32, fp16 and bf16 logits; there is no fallback.
 """
 import functools
 from typing import Optional
@@ -974,7 +975,8 @@ def distill_loss(logits, values, indices, targets, padidx, tail=None, temperatur
 
     reduction: "mean" over the rows that count (0 if there are none), "sum", or "none" (a loss per row).  Differentiable
     in the logits alone.  ``eager_grad=False`` for a scalar loss that will be scaled before its backward -- by a gradient
-    scaler, a number of accumulation steps -- : the gradient is then computed in the backward only, see RowLossFn."""
+    scaler, a number of accumulation steps -- : the gradient is then computed in the backward only, see RowLossFn.
+    The divergence is a difference of fp32 sums' logarithms: off by some 2^-20, times temperature^2 in the loss."""
     args = (targets, values, indices, padidx, tail, temperature, ce_weight)
     if _grad_wanted(logits):
         return RowLossFn.apply(logits, (_DistillLoss, args, reduction, eager_grad))
