@@ -1360,6 +1360,7 @@ __global__ __launch_bounds__(1024) void prefer_kernel(Prefer a)
         const int64_t b = b0 + lane;
         double s = 0.0;
         if (b < S && g < G)
+#pragma unroll 8
             for (int64_t t = g; t < a.T; t += G) s += a.logp[a.batch_first ? b * a.T + t : t * S + b];
         part[threadIdx.x] = s;
         __syncthreads();

@@ -392,6 +392,17 @@ def test_distill_lists_with_gaps_repeats_and_masks(dtype):
     assert torch.isnan(_fn().distill_loss(xg, v.cuda(), far.cuda(), y.cuda(), 0))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_distill_at_the_largest_vocabulary(dtype):
+    V, k = 400000, 256
+    x, y, g = _logits(1, 2, V, dtype, seed=8)
+    v, i, t = _teacher(x, k, 2.0, g, dtype)
+    i = i.clone()
+    i[0, 0, 0], i[0, 1, 255] = V - 1, 0
+    y[0, 0], y[0, 1] = V - 1, int(i[0, 1, 3])
+    _check_distill(x, y, v, i, t, 2.0, 0.5)
+
+
 def test_distill_student_far_below_the_teachers_tail():
     # nearly all of the student's mass on the list, the rest 100 below: p_t is e^-100 and still has its relative precision
     V, k = 400, 4
