@@ -531,16 +531,17 @@ struct Scale {
         mu = 0.f;
     }
     __device__ __forceinline__ float y(float x) const { return fmaf(x, c, -mu); }
-    // in 64 bits and units of e: the log of a logit's exponential relative to the sums' reference
-    __device__ __forceinline__ double log_of(float x, double inv_tau) const
+    // in 64 bits and units of e: the log of a logit's exponential relative to the sums' reference.  With the rounded c, like the
+    // sums: a soft-max whose temperature is 2^-25 off is a soft-max still, and a divergence near zero stays near zero.
+    __device__ __forceinline__ double log_of(float x) const
     {
-        return flat ? ((double)x - (double)m) * inv_tau : fma((double)x, (double)c, -(double)mu) * LN2;
+        return flat ? ((double)x - (double)m) * (double)c * LN2 : fma((double)x, (double)c, -(double)mu) * LN2;
     }
     // the sums' own reference relative to another logit `to`, likewise
-    __device__ __forceinline__ double log_ref(float to, double inv_tau) const
+    __device__ __forceinline__ double log_ref(float to) const
     {
         if (m == neg_inf()) return -__builtin_inf();
-        return flat ? ((double)m - (double)to) * inv_tau : fma(-(double)to, (double)c, (double)mu) * LN2;
+        return flat ? ((double)m - (double)to) * (double)c * LN2 : fma(-(double)to, (double)c, (double)mu) * LN2;
     }
     // this reference minus another's, in powers of two
     __device__ __forceinline__ float above(const Scale& o) const
@@ -688,7 +689,7 @@ __global__ __launch_bounds__(NT, min_waves(NV)) void logprob_kernel(Rows rows, d
     if (threadIdx.x == 0) {
         const int64_t y = rows.targets[r];
         const double log_s = log_row((double)a.s), u = -(double)a.t / (double)a.s * LN2;
-        const double lp = (y >= 0 && y < rows.vocab) ? sc.log_of(E::load(x + y), inv_tau) - log_s : __builtin_nan("");
+        const double lp = (y >= 0 && y < rows.vocab) ? sc.log_of(E::load(x + y)) - log_s : __builtin_nan("");
         if (out.logp) out.logp[r] = (float)lp;
         if (out.entropy) out.entropy[r] = (float)(log_s + u);
         if (out.logp64) out.logp64[r] = lp;
@@ -823,7 +824,7 @@ __global__ __launch_bounds__(NT, min_waves(NV)) void policy_kernel(Rows rows, Po
     const int y = (y64 >= 0 && y64 < rows.vocab) ? (int)y64 : -1;
     if (threadIdx.x < 64) {
         const double it = a.inv_tau, log_s = log_row((double)s), u = -(double)t / (double)s * LN2, H = log_s + u;
-        const double lp = y >= 0 ? sc.log_of(E::load(x + y), it) - log_s : __builtin_nan("");
+        const double lp = y >= 0 ? sc.log_of(E::load(x + y)) - log_s : __builtin_nan("");
         const double A = (double)a.adv[r % a.adv_rows], gap = a.ref_logp ? (double)a.ref_logp[r] - lp : 0.0;
         // two exponentials, side by side in two lanes
         const double both = exp_row(threadIdx.x == 0 ? lp - (double)a.old_logp[r] : gap);
@@ -963,7 +964,7 @@ __global__ __launch_bounds__(NT, min_waves(NV)) void distill_kernel(Rows rows, D
 
     // one wave: the teacher's distribution, the student's sums over everything, the loss
     if (tid < 64) {
-        const double it = a.inv_tau;
+        const double it = a.inv_tau, its = (double)c * LN2, its1 = (double)c1 * LN2;  // the teacher's; the student's, see Scale
         const double tail = a.tail ? (double)a.tail[r] : -(double)__builtin_inff();
         float tm = neg_inf(), xm = m_rest;
         for (int k = tid; k < a.k; k += 64) {
@@ -980,7 +981,7 @@ __global__ __launch_bounds__(NT, min_waves(NV)) void distill_kernel(Rows rows, D
             const float q = exp2_raw((float)((u - M) * LOG2E));
             sq[k] = q;
             z += (double)q;
-            if (q != 0.f) cross += (double)q * ((u - M) - ((double)sx[k] - (double)m) * it);
+            if (q != 0.f) cross += (double)q * ((u - M) - ((double)sx[k] - (double)m) * its);
             if (own[k]) {
                 s += (double)exp2_raw((sx[k] - m) * c);
                 if (BOTH) s1 += (double)exp2_raw((sx[k] - m) * c1);
@@ -992,7 +993,7 @@ __global__ __launch_bounds__(NT, min_waves(NV)) void distill_kernel(Rows rows, D
         cross = wave_sum(cross);
         // exponentials and logarithms side by side in the wave's lanes; those that scale every class outside the list,
         // of (the others' reference) - (the row's maximum), in 64 bits like the rest
-        const double gap = sc.log_ref(m, it), gap1 = BOTH ? sc1.log_ref(m, 1.0) : gap;
+        const double gap = sc.log_ref(m), gap1 = BOTH ? sc1.log_ref(m) : gap;
         const double e3 = exp_row(tid == 0 ? tail - M : tid == 1 ? gap : gap1);
         const double qt0 = lane_value(e3, 0), lift = lane_value(e3, 1), lift1 = BOTH ? lane_value(e3, 2) : lift;
         z += qt0;
@@ -1011,7 +1012,7 @@ __global__ __launch_bounds__(NT, min_waves(NV)) void distill_kernel(Rows rows, D
             kd *= wkd * a.tau * a.tau;
         }
         double ce = 0.0;
-        if (a.ce != 0.0 && y >= 0) ce = a.ce * (log_s1 - ((double)E::load(x + y) - (double)m));
+        if (a.ce != 0.0 && y >= 0) ce = a.ce * (log_s1 - ((double)E::load(x + y) - (double)m) * its1);
         if (tid == 0) {
             double loss = kd + ce;
             if (bad) loss = __builtin_nan("");
