@@ -1401,7 +1401,9 @@ __global__ __launch_bounds__(1024) void prefer_kernel(Prefer a)
 // 256 threads, 45 with 64; policy loss 154 and 92; the k largest 200 and 140).  From 513 to 1024 two waves, but one for the
 // k largest, which has no LDS to wait for then: 40 000 rows of 2500 fp32 169 and 142 us; the distillation 187 with two, 198 with one.
 // One wave is slow to rank a long list, though: above k = 64 the rows of 257 to 1024 vectors take four (k = 256, 20 000 rows of
-// 4000 fp32: 635 us with one, 406 with four; k = 64 141 and 130, and of 2000 fp32 207 and 238).
+// 4000 fp32: 635 us with one, 406 with four; k = 64 141 and 130, and of 2000 fp32 207 and 238).  Longer rows than registers hold
+// are read again in every sweep, by 1024 threads (1500 rows of 150 000 bf16, policy loss: 256 threads 284 us, 512 247, 1024 215;
+// 16 rows: 63, 37, 32).  Registers where they hold the row all the same: distillation of 1533 rows of 131 072 bf16 170 us, streamed 185.
 template <typename E_, int NT_, int NV_>
 struct Shape {
     typedef E_ E;
@@ -1418,7 +1420,7 @@ void by_vectors(int64_t n, F launch)
     else if (n <= 4096) launch(Shape<E, 512, 8>());
     else if (n <= 8192) launch(Shape<E, 512, 16>());
     else if (n <= 16384) launch(Shape<E, 1024, 16>());
-    else launch(Shape<E, 512, 0>());
+    else launch(Shape<E, 1024, 0>());
 }
 template <int MID = 128, typename F>
 void by_size(int dtype, int vocab, F launch)
