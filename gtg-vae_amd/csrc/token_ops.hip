@@ -1063,9 +1063,11 @@ __device__ __forceinline__ unsigned order_key(float x)
 // The usual way takes two sweeps.  The first finds maxima of parts of the row, one per thread (two, of halves of its vectors,
 // for a k that is not small beside the threads; up to eight where one wave has the row): the k-th largest of them is a bound
 // that at least k elements reach and few more do.  The second puts what reaches the bound on a list and sums the exponentials
-// of everything below, relative to the bound.  The list's elements then find their rank by comparing with each other.  Where the list would overflow (many equal
-// values), or a NaN is about, the k-th largest is found bit by bit with a sweep for each; where what lies below the bound
-// vanishes beside it, the tail is summed in two more sweeps relative to its own maximum.
+// of everything below, relative to the bound.  The list's elements then find their rank by comparing with each other.
+// Where what lies below the bound vanishes beside it, the tail is summed in two more sweeps relative to its own maximum.
+// Where the list would overflow (many equal values) or a NaN is about: a row that is its lowest value but for few elements (a
+// mask's rows; all equal ones) has the k largest among those and its first k elements; in any other the k-th largest is found bit
+// by bit with a sweep for each, 65 in all (10 240 rows of 30 522 bf16, 50 classes not masked: 64 largest 619 us so, 4121 bit by bit).
 
 __device__ __forceinline__ float key_value(unsigned key)  // the float of a key that is no NaN's
 {
@@ -1232,31 +1234,42 @@ __global__ __launch_bounds__(NT, NT == 64 ? 3 : NT == 256 ? 6 : NV == 8 ? 8 : mi
             });
             return block_sum<NT, true>(cnt, sh);
         };
-        unsigned kth = 0;  // the largest key that at least k elements reach
-        for (int bit = 31; bit >= 0; --bit) {
-            const unsigned cand = kth | (1u << bit);
-            if (count([&](int, float v) { return order_key(v) >= cand; }) >= k) kth = cand;
-        }
-        const int need = k - count([&](int, float v) { return order_key(v) > kth; });
-        int last = 0;  // the need-th element of that key, by index
-        for (int bit = 30; bit >= 0; --bit) {
-            const int cand = last + (1 << bit);
-            if (cand < V && count([&](int j, float v) { return j < cand && order_key(v) == kth; }) < need) last = cand;
-        }
         __syncthreads();
         if (tid == 0) fill = 0;
         __syncthreads();
+        // Rows of which most is one lowest value (a mask's): what is above it and the first k elements hold the k largest.
+        float low = again.je >= 0 ? again.xe : __builtin_inff();
+        again.template each<false>([&](int, const u32x4& v) {
+#pragma unroll
+            for (int q = 0; q < E::VEC; ++q) low = fminf(low, E::get(v, q));
+        });
+        low = block_reduce<NT, true>(low, shf, [](float a, float b) { return fminf(a, b); });
+        auto above = [&](int j, float v) { return j < k || !(v <= low); };
+        const int few = count(above);
+        unsigned kth = 0;  // the largest key that at least k elements reach
+        int last = 0;      // the last one of that key, by index, that is taken
         auto take = [&](int j, float f) {
             const unsigned key = order_key(f);
-            if (key > kth || (key == kth && j <= last)) put(atomicAdd(&fill, 1), j, f);
+            if (few <= TOP_LIST ? above(j, f) : key > kth || (key == kth && j <= last)) put(atomicAdd(&fill, 1), j, f);
         };
+        if (few > TOP_LIST) {
+            for (int bit = 31; bit >= 0; --bit) {
+                const unsigned cand = kth | (1u << bit);
+                if (count([&](int, float v) { return order_key(v) >= cand; }) >= k) kth = cand;
+            }
+            const int need = k - count([&](int, float v) { return order_key(v) > kth; });
+            for (int bit = 30; bit >= 0; --bit) {
+                const int cand = last + (1 << bit);
+                if (cand < V && count([&](int j, float v) { return j < cand && order_key(v) == kth; }) < need) last = cand;
+            }
+        }
         if (again.je >= 0) take(again.je, again.xe);
         again.template each<false>([&](int j, const u32x4& v) {
 #pragma unroll
             for (int q = 0; q < E::VEC; ++q) take(j + q, E::get(v, q));
         });
         __syncthreads();
-        n = k;
+        n = fill;
     }
     // ranks: a wave compares 64 of the list's elements with its share of the whole list
     {

@@ -141,6 +141,29 @@ def test_top_logits_of_many_out_of_few(V, dtype):
         _check_top(x, k)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [300, 1500, 9001, 30522, 140003])
+def test_top_logits_of_masked_vocabularies(V, dtype):
+    """Rows of which a mask leaves few classes: fewer than k, about as many, all in one place, or none."""
+    g = torch.Generator().manual_seed(V)
+    rows = []
+    for mask in (-math.inf, torch.finfo(dtype).min, -1e4, 0.0):
+        for keep in (torch.randperm(V, generator=g)[:10], torch.randperm(V, generator=g)[:100], torch.arange(V - 150, V), torch.arange(70, 90),
+                     torch.arange(1)):
+            r = torch.full((V,), mask)
+            r[keep] = torch.randn(keep.numel(), generator=g).abs()
+            rows.append(r)
+        nan = rows[-1].clone()
+        nan[V // 2] = math.nan
+        rows.append(nan)
+        both = rows[-5].clone()                  # two kinds of masked places
+        both[: V // 2] = torch.where(both[: V // 2] == mask, -2e4, both[: V // 2])
+        rows.append(both)
+    x = torch.stack(rows).to(dtype)
+    for k in (1, 20, 64, 256):
+        _check_top(x, k)
+
+
 def test_top_logits_takes_strides_and_other_shapes():
     Fn = _fn()
     x, _, _ = _logits(6, 5, 1003, torch.bfloat16, seed=1)
